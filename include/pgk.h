@@ -142,6 +142,75 @@ PG_API int pgk_gather(void *const *dsts, const void *const *srcs, const size_t *
 PG_API int pgk_all_reduce_staged(void *const *sendbufs, void *const *recvbufs, int world, size_t count,
                                  int rings, int dt, int op, void *stream);
 
+/* ---- gradients of a data-parallel training step -----------------------------
+ *
+ * No counterpart in the reference.  What a training step does with gradients
+ * beside a reduction over the ranks: average the ranks' copies (pgk_grad_fold),
+ * take the global norm over all tensors (pgk_grad_sumsq), clip by it
+ * (pgk_grad_clip).  pg_grad_clip (include/pg_ext.h) is the same over the ranks
+ * of a process group.
+ *
+ * Types: the two values above are joined by f32, f16 and bf16.  Gradients are
+ * PGK_DT_DOUBLE, _F32, _F16 or _BF16 (int32 is refused).  Outputs have the
+ * gradients' type, or PGK_DT_F32 for f16 / bf16 gradients (the 32-bit copy an
+ * optimizer keeps).  The other entry points of this header take int32 and
+ * double only.
+ *
+ * Tensors are contiguous, on a multiple of their element size (16-byte
+ * alignment is not needed), up to 2^40 elements each; a tensor of 0 elements is
+ * skipped and its pointer may be NULL.  Elements between and behind the tensors
+ * are neither read nor written.  Any number of tensors: a launch holds 180 of
+ * them (pgk_grad_sumsq) or 128 (pgk_grad_clip).
+ *
+ * work: PGK_GRAD_WORK_BYTES of device memory, 8-byte aligned, any contents.  A
+ * call uses it until it has run on its stream; calls that may overlap in time
+ * (two streams, two graphs replayed at once) need one each.
+ *
+ * Results depend on the values, the sizes and the order of the tensors and the
+ * GPU's number of CUs only: the same call gives the same bits. */
+#define PGK_DT_F32  2
+#define PGK_DT_F16  3
+#define PGK_DT_BF16 4
+#define PGK_GRAD_WORK_BYTES 65536
+
+/* *sumsq (device) = the sum of the squares of all elements of the k tensors,
+ * formed and summed in 64 bits: no f32, f16 or bf16 value overflows or
+ * underflows in it.  A NaN or an infinity among the gradients gives NaN or
+ * infinity.  No tensors, or empty ones only: 0.  The gradient norm is its
+ * square root; pgk_grad_clip forms it.  One type per call: tensors of several
+ * types take a call and a place in a sumsq array each. */
+PG_API int pgk_grad_sumsq(const void *const *grads, const size_t *ns, int k, int dt, double *sumsq, void *work,
+                          void *stream);
+
+/* Clip by the global norm.  With S = sumsq[0] + ... + sumsq[nsum-1] (device):
+ *     norm = |scale| * sqrt(S)
+ *     c = scale * min(1, max_norm / (norm + 1e-6))
+ *     outs[j][i] = c * grads[j][i]     for i < ns[j], j < k
+ * scale (finite) is what the gradients are multiplied by in any case: 1, the
+ * 1 / world_size of a mean, the inverse of a loss scale.  max_norm >= 0;
+ * infinity does not clip.  *norm (device, may be NULL) receives the norm, also
+ * when k = 0.  f64 and f32 results are rounded once, from a 64-bit product;
+ * f16 and bf16 ones from a 32-bit product.
+ * A norm that is not finite clips as the formula says: an infinite one gives 0,
+ * and NaN where the gradient is infinite; NaN gives NaN everywhere.  A caller
+ * who would rather skip such a step looks at *norm first.
+ * outs[j] == grads[j] (in place) is allowed when the types are equal; other
+ * overlaps are not (within a pair they are refused), nor is a tensor that is
+ * listed twice. */
+PG_API int pgk_grad_clip(void *const *outs, int out_dt, const void *const *grads, int dt, const size_t *ns, int k,
+                         const double *sumsq, int nsum, double scale, double max_norm, double *norm, void *stream);
+
+/* The averaging fold: out[i] = scale * (srcs[0][i] + srcs[1][i] + ... +
+ * srcs[nsrc-1][i]) for i < n, 1 <= nsrc <= 16, summed left to right in 64 bits
+ * and rounded to the output's type at the end (f16 and bf16 by way of f32).
+ * scale (finite): 1, or 1 / nsrc for the mean.
+ * sumsq (device, may be NULL): the sum of the squares of out as stored, what
+ * pgk_grad_sumsq over out would give up to the order of its sum, without reading
+ * it again.  Without sumsq, work may be NULL.  n = 0 gives 0.  Sources may be peer GPUs' memory as in
+ * pgk_reduce_multi; out may be one of them when the types are equal. */
+PG_API int pgk_grad_fold(void *out, int out_dt, const void *const *srcs, int nsrc, size_t n, int dt, double scale,
+                         double *sumsq, void *work, void *stream);
+
 /* Device helpers for hosts that do not link HIP themselves (ctypes, cgo ...). */
 PG_API int pgk_device_count(int *count);
 PG_API int pgk_set_device(int device);

@@ -23,6 +23,7 @@
 #include <string.h>
 
 #include "pgk.h"
+#include "pgk_impl.h"
 
 namespace {
 
@@ -384,12 +385,18 @@ __global__ __launch_bounds__(kMultiBlock) void k_gather(CopyList cl) {
 
 thread_local char g_err[256] = "";
 
-void set_err(const char* fmt, ...) {
+}  // namespace
+
+void pgk_set_err(const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_err, sizeof(g_err), fmt, ap);
   va_end(ap);
 }
+
+namespace {
+
+#define set_err pgk_set_err
 
 // Tuning (process-wide).  The defaults are the measured best on MI355X (the figures are beside each knob).
 int g_blocks_per_cu = 0;   // one-shot grid: 6403 vs 6200 GB/s capped at 8/CU (sweep r01)
@@ -426,6 +433,12 @@ int cu_count() {
   }
   return g_cu_count[dev];
 }
+
+}  // namespace
+
+int pgk_cu_count() { return cu_count(); }
+
+namespace {
 
 // The AQL dispatch packet holds the grid size in WORK-ITEMS as 32 bits, so
 // gridDim.x * blockDim.x must stay below 2^32; the kernels grid-stride over

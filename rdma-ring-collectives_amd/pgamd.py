@@ -28,6 +28,8 @@ PG_BUF_NONE, PG_BUF_SRC, PG_BUF_OUT, PG_BUF_STAGE0, PG_BUF_STAGE1 = 0, 1, 2, 3, 
 PG_COLL_REDUCE_SCATTER, PG_COLL_ALL_GATHER, PG_COLL_ALL_REDUCE = 0, 1, 2
 # include/pgk.h
 PGK_STAGED_MAX_BYTES = 16 << 20
+DT_F32, DT_F16, DT_BF16 = 2, 3, 4                  # gradient types of pgk_grad_* beside DT_DOUBLE
+PGK_GRAD_WORK_BYTES = 65536
 
 ELEM_SIZE = {DT_INT32: 4, DT_DOUBLE: 8}
 
@@ -124,6 +126,10 @@ _SIGS = {
     "pgk_fold_blocks": (_I, [_VP, ctypes.POINTER(_VP), _I, _SZ, _SZ, _I, _I, _I, _VP]),
     "pgk_gather": (_I, [ctypes.POINTER(_VP), ctypes.POINTER(_VP), ctypes.POINTER(_SZ), _I, _VP]),
     "pgk_all_reduce_staged": (_I, [ctypes.POINTER(_VP), ctypes.POINTER(_VP), _I, _SZ, _I, _I, _I, _VP]),
+    "pgk_grad_sumsq": (_I, [ctypes.POINTER(_VP), ctypes.POINTER(_SZ), _I, _I, _VP, _VP, _VP]),
+    "pgk_grad_clip": (_I, [ctypes.POINTER(_VP), _I, ctypes.POINTER(_VP), _I, ctypes.POINTER(_SZ), _I, _VP, _I,
+                           ctypes.c_double, ctypes.c_double, _VP, _VP]),
+    "pgk_grad_fold": (_I, [_VP, _I, ctypes.POINTER(_VP), _I, _SZ, _I, ctypes.c_double, _VP, _VP, _VP]),
     "pgk_device_count": (_I, [ctypes.POINTER(_I)]),
     "pgk_set_device": (_I, [_I]),
     "pgk_synchronize": (_I, []),
