@@ -184,12 +184,16 @@ def _plain_fold(srcs, out):
 
 # ---- one pass --------------------------------------------------------------------------------------
 
+_loaded = []
+
+
 def _library():
-    at = str(pathlib.Path(__file__).resolve().parents[1] / "rdma-ring-collectives_amd")
-    if at not in sys.path:
-        sys.path.insert(0, at)
-    import pgamd
-    return pgamd, pgamd.load()
+    """The binding and the library, loaded by the first call as a program's import does."""
+    if not _loaded:
+        sys.path.insert(0, str(pathlib.Path(__file__).resolve().parents[1] / "rdma-ring-collectives_amd"))
+        import pgamd
+        _loaded.extend((pgamd, pgamd.load()))
+    return _loaded
 
 
 def _own_sumsq(state):
