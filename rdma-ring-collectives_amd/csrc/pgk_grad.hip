@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "pgk.h"
 #include "pgk_impl.h"
@@ -27,37 +28,30 @@ namespace {
 
 // ---- element types -----------------------------------------------------------
 
-// Wide is what the clip product is formed in: 64 bits where the result keeps
-// 24 bits or more (one rounding, to the stored type), 32 bits for a 16-bit result.
-template <int DT> struct Type;
-template <> struct Type<PGK_DT_DOUBLE> { using T = double; };
-template <> struct Type<PGK_DT_F32> { using T = float; };
-template <> struct Type<PGK_DT_F16> { using T = _Float16; };
-template <> struct Type<PGK_DT_BF16> { using T = __bf16; };
-
-// 16 bytes of T at any element's address: gfx950 loads and stores 16 bytes at
-// every alignment, so a tensor may start at any element of a bucket.
+// N elements at any element's address, up to 16 bytes: gfx950 loads and stores
+// them at every alignment, so a tensor may start at any element of a bucket.
+// Non-temporal (nothing here is read twice by one launch): a read-only pass over
+// 1.3 GB runs at 7.0 TB/s against 6.2 with the default policy, a scaled copy of
+// 1.07 GB at 6.4 against 5.85.
 template <typename T> constexpr int kWidth = 16 / (int)sizeof(T);
-template <typename T, int N> struct Pack { T v[N]; };
-template <typename T, int N> using VecT = T __attribute__((ext_vector_type(N)));
 
 template <typename T, int N>
 __device__ __forceinline__ void load(T (&x)[N], const T* p) {
-  using V = VecT<T, N>;
+  typedef T V __attribute__((ext_vector_type(N)));
   typedef V VU __attribute__((aligned(sizeof(T))));
-  const V v = *reinterpret_cast<const VU*>(p);
+  const V v = __builtin_nontemporal_load(reinterpret_cast<const VU*>(p));
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = v[i];
 }
 
 template <typename T, int N>
 __device__ __forceinline__ void store(T* p, const T (&x)[N]) {
-  using V = VecT<T, N>;
+  typedef T V __attribute__((ext_vector_type(N)));
   typedef V VU __attribute__((aligned(sizeof(T))));
   V v;
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = x[i];
-  *reinterpret_cast<VU*>(p) = v;
+  __builtin_nontemporal_store(v, reinterpret_cast<VU*>(p));
 }
 
 template <typename T>
@@ -83,33 +77,34 @@ __device__ __forceinline__ O from_f64(double x) {
 // ---- lists of tensors ------------------------------------------------------------
 
 // A launch takes its tensors by value: no table to keep, nothing to copy, and a
-// captured graph holds them.  4 KiB of kernel arguments (the runtime adds its own) bound the number.
-constexpr int kBlock = 256;
-constexpr int kTileVecs = 4;                      // 16-byte vectors per thread and tile
-constexpr int kMaxRead = 180;                     // tensors per launch, read only
-constexpr int kMaxCopy = 128;                     // tensors per launch, read and written
-constexpr int kMaxGrid = PGK_GRAD_WORK_BYTES / 8; // one partial sum per block
-
-template <typename T> constexpr unsigned kTile = kBlock * kTileVecs * kWidth<T>;   // elements
+// captured graph holds them.  4 KiB of kernel arguments (the runtime adds its
+// own) bound the number.  A tile is what a block takes at a time; every tensor
+// starts a tile.  A tensor of more than 2^31 elements is listed in pieces.
+constexpr int kMaxRead = 250;                     // tensors per launch, read only
+constexpr int kMaxCopy = 160;                     // tensors per launch, read and written
+constexpr size_t kMaxPiece = (size_t)1 << 31;
+constexpr int kMaxParts = PGK_GRAD_WORK_BYTES / 8;   // partial sums that the workspace holds
 
 template <int K>
 struct ReadList {
+  static constexpr int kMost = K;
   const void* p[K];
-  size_t n[K];
+  unsigned n[K];
   unsigned first[K + 1];                          // tile at which each tensor starts
   int k;
 };
 
 template <int K>
 struct CopyList {
+  static constexpr int kMost = K;
   const void* p[K];
   void* out[K];
-  size_t n[K];
+  unsigned n[K];
   unsigned first[K + 1];
   int k;
 };
 
-// The tensor that tile t lies in, at or after j.
+// The tensor that tile t lies in.
 template <typename L>
 __device__ __forceinline__ int find(const L& l, unsigned t) {
   int lo = 0, hi = l.k - 1;
@@ -141,127 +136,219 @@ __device__ __forceinline__ double block_sum(double x) {
   return x;
 }
 
-// ---- kernels ---------------------------------------------------------------------
+// A block's share of the sum goes to its own place; the places below `held` have
+// the shares of the call's earlier launches in them, the others anything.
+template <int BLOCK>
+__device__ __forceinline__ void keep(double* parts, int held, double x) {
+  x = block_sum<BLOCK>(x);
+  if (threadIdx.x == 0) parts[blockIdx.x] = (int)blockIdx.x < held ? parts[blockIdx.x] + x : x;
+}
 
-template <typename T>
-__global__ __launch_bounds__(kBlock) void k_grad_sumsq(ReadList<kMaxRead> l, double* parts, int add) {
+template <typename T, int N>
+__device__ __forceinline__ double squares(const T (&x)[N], double acc) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc = fma(to_f64(x[i]), to_f64(x[i]), acc);
+  return acc;
+}
+
+// ---- sum of squares ----------------------------------------------------------------
+
+// A stream of reads, 16 bytes x UNROLL in flight per thread; the f64 conversions
+// and products hide behind it (accumulating in 32 bits takes the same time).
+template <typename T, int BLOCK, int UNROLL>
+__global__ __launch_bounds__(BLOCK) void k_grad_sumsq(ReadList<kMaxRead> l, double* parts, int held) {
   constexpr int W = kWidth<T>;
+  constexpr unsigned kTile = BLOCK * UNROLL * W;
   double acc = 0.0;
   const unsigned tiles = l.first[l.k];
+  int j = 0;
+  unsigned begin = 0, end = 0;                    // the tiles of tensor j
   for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int j = find(l, t);
-    const size_t at = (size_t)(t - l.first[j]) * kTile<T>;
+    if (t >= end) {
+      j = find(l, t);
+      begin = l.first[j];
+      end = l.first[j + 1];
+    }
+    const unsigned at = (t - begin) * kTile, left = l.n[j] - at;
     const T* p = (const T*)l.p[j] + at;
-    const size_t left = l.n[j] - at;
-    for (unsigned e = threadIdx.x * W; e < kTile<T>; e += kBlock * W) {
-      if (e + W <= left) {
-        T x[W];
-        load(x, p + e);
+    if (left >= kTile) {
+      T x[UNROLL][W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) acc = fma(to_f64(x[i]), to_f64(x[i]), acc);
-      } else {
-        for (unsigned i = e; i < left; ++i) acc = fma(to_f64(p[i]), to_f64(p[i]), acc);
+      for (int u = 0; u < UNROLL; ++u) load(x[u], p + (u * BLOCK + threadIdx.x) * W);
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) acc = squares(x[u], acc);
+    } else {
+      for (unsigned e = threadIdx.x * W; e < left; e += BLOCK * W) {
+        if (e + W <= left) {
+          T x[W];
+          load(x, p + e);
+          acc = squares(x, acc);
+        } else {
+          for (unsigned i = e; i < left; ++i) acc = fma(to_f64(p[i]), to_f64(p[i]), acc);
+        }
       }
     }
   }
-  acc = block_sum<kBlock>(acc);
-  if (threadIdx.x == 0) parts[blockIdx.x] = add ? parts[blockIdx.x] + acc : acc;
+  keep<BLOCK>(parts, held, acc);
 }
 
-__global__ __launch_bounds__(1024) void k_grad_finish(const double* parts, int n, double* sumsq) {
+constexpr int kFinishBlock = 1024;
+__global__ __launch_bounds__(kFinishBlock) void k_grad_finish(const double* parts, int n, double* sumsq) {
   double acc = 0.0;
-  for (int i = threadIdx.x; i < n; i += 1024) acc += parts[i];
-  acc = block_sum<1024>(acc);
+  for (int i = threadIdx.x; i < n; i += kFinishBlock) acc += parts[i];
+  acc = block_sum<kFinishBlock>(acc);
   if (threadIdx.x == 0) *sumsq = acc;
 }
 
-// c, and the norm it is formed from.  Every block forms the same bits.
+// ---- clip --------------------------------------------------------------------------
+
+// c, and the norm it is formed from.  Every wave forms the same bits.
 __device__ __forceinline__ double coefficient(const double* sumsq, int nsum, double scale, double max_norm,
                                               double* norm) {
   double s = 0.0;
-  for (int j = 0; j < nsum; ++j) s += sumsq[j];
+  if (nsum == 1) {
+    s = sumsq[0];
+  } else {
+    for (int j = threadIdx.x & 63; j < nsum; j += 64) s += sumsq[j];
+    s = wave_sum(s);
+  }
   *norm = fabs(scale) * sqrt(s);
   const double c = max_norm / (*norm + 1e-6);
   return scale * (c > 1.0 ? 1.0 : c);              // a NaN stays one
 }
 
+// What the product is formed in: 64 bits where the result keeps 24 bits or more
+// (one rounding, to the stored type), 32 bits for a 16-bit result.
 template <typename O, typename T>
-__device__ __forceinline__ O scaled(T x, double c, float cf) {
-  if constexpr (sizeof(O) == 2) return (O)((float)x * cf);
+__device__ __forceinline__ O scaled(T x, double c) {
+  if constexpr (sizeof(O) == 2) return (O)((float)x * (float)c);
   else return (O)(to_f64(x) * c);
 }
 
+// One tile per block, one vector per thread: blocks that come and go keep reads
+// and writes mixed (a grid that loops streams 10-15% slower).  A vector is 16
+// bytes of the wider type: a lane that stores two halves of 32 bytes leaves
+// every store instruction with gaps (5.4 against 6.5 TB/s).
+constexpr int kClipBlock = 1024;
+template <typename T, typename O> constexpr int kPair = sizeof(T) > sizeof(O) ? kWidth<T> : kWidth<O>;
+
 template <typename T, typename O>
-__global__ __launch_bounds__(kBlock) void k_grad_clip(CopyList<kMaxCopy> l, const double* sumsq, int nsum,
-                                                      double scale, double max_norm, double* norm) {
-  constexpr int W = kWidth<T>;
+__global__ __launch_bounds__(kClipBlock) void k_grad_clip(CopyList<kMaxCopy> l, const double* sumsq, int nsum,
+                                                          double scale, double max_norm, double* norm) {
+  constexpr int W = kPair<T, O>;
+  constexpr unsigned kTile = kClipBlock * W;
   double nrm;
+  if (l.first[l.k] == 0) {                         // no elements: the norm alone
+    coefficient(sumsq, nsum, scale, max_norm, &nrm);
+    if (threadIdx.x == 0) *norm = nrm;
+    return;
+  }
+  const int j = find(l, blockIdx.x);
+  const unsigned at = (blockIdx.x - l.first[j]) * kTile, left = l.n[j] - at, e = threadIdx.x * W;
+  const T* p = (const T*)l.p[j] + at;
+  O* o = (O*)l.out[j] + at;
+  T x[W];
+  const bool whole = e + W <= left;
+  if (whole) load(x, p + e);                       // on its way while c is formed
   const double c = coefficient(sumsq, nsum, scale, max_norm, &nrm);
-  const float cf = (float)c;
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = nrm;
-  const unsigned tiles = l.first[l.k];
-  for (unsigned t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int j = find(l, t);
-    const size_t at = (size_t)(t - l.first[j]) * kTile<T>;
-    const T* p = (const T*)l.p[j] + at;
-    O* o = (O*)l.out[j] + at;
-    const size_t left = l.n[j] - at;
-    for (unsigned e = threadIdx.x * W; e < kTile<T>; e += kBlock * W) {
-      if (e + W <= left) {
-        T x[W];
-        O y[W];
-        load(x, p + e);
+  if (whole) {
+    O y[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) y[i] = scaled<O>(x[i], c, cf);
-        store(o + e, y);
-      } else {
-        for (unsigned i = e; i < left; ++i) o[i] = scaled<O>(p[i], c, cf);
-      }
-    }
+    for (int i = 0; i < W; ++i) y[i] = scaled<O>(x[i], c);
+    store(o + e, y);
+  } else {
+    for (unsigned i = e; i < left; ++i) o[i] = scaled<O>(p[i], c);
   }
 }
 
+// ---- averaging fold ------------------------------------------------------------------
+
 constexpr int kMaxSrc = 16;
+constexpr int kMaxUnrolled = 8;                   // sources whose loads are all in flight at once
 struct Sources { const void* p[kMaxSrc]; };
 
-template <typename T, typename O>
-__global__ __launch_bounds__(kBlock) void k_grad_fold(O* out, Sources src, int nsrc, size_t n, double scale,
-                                                      double* parts) {
-  constexpr int W = kWidth<T>;
-  double sq = 0.0;
-  const size_t stride = (size_t)gridDim.x * kBlock * W;
-  for (size_t e = ((size_t)blockIdx.x * kBlock + threadIdx.x) * W; e < n; e += stride) {
-    if (e + W <= n) {
-      double acc[W];
-      T x[W];
-      load(x, (const T*)src.p[0] + e);
+// The mean of W elements at e, summed left to right; its squares into sq.
+template <typename T, typename O, int NS, int W>
+__device__ __forceinline__ void fold(O (&y)[W], const Sources& src, int nsrc, size_t e, double scale, double* sq) {
+  T x[NS][W];
 #pragma unroll
-      for (int i = 0; i < W; ++i) acc[i] = to_f64(x[i]);
-      for (int s = 1; s < nsrc; ++s) {
-        load(x, (const T*)src.p[s] + e);
+  for (int s = 0; s < NS; ++s) load(x[s], (const T*)src.p[s] + e);
+  double acc[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) acc[i] += to_f64(x[i]);
-      }
-      O y[W];
+  for (int i = 0; i < W; ++i) acc[i] = to_f64(x[0][i]);
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        y[i] = from_f64<O>(acc[i] * scale);
-        sq = fma(to_f64(y[i]), to_f64(y[i]), sq);
-      }
-      store(out + e, y);
-    } else {
-      for (size_t i = e; i < n; ++i) {
-        double acc = to_f64(((const T*)src.p[0])[i]);
-        for (int s = 1; s < nsrc; ++s) acc += to_f64(((const T*)src.p[s])[i]);
-        const O y = from_f64<O>(acc * scale);
-        sq = fma(to_f64(y), to_f64(y), sq);
-        out[i] = y;
-      }
+  for (int s = 1; s < NS; ++s)
+#pragma unroll
+    for (int i = 0; i < W; ++i) acc[i] += to_f64(x[s][i]);
+  if constexpr (NS == kMaxUnrolled) {
+#pragma unroll 4
+    for (int s = NS; s < nsrc; ++s) {
+      T z[W];
+      load(z, (const T*)src.p[s] + e);
+#pragma unroll
+      for (int i = 0; i < W; ++i) acc[i] += to_f64(z[i]);
     }
   }
-  if (!parts) return;
-  sq = block_sum<kBlock>(sq);
-  if (threadIdx.x == 0) parts[blockIdx.x] = sq;
+#pragma unroll
+  for (int i = 0; i < W; ++i) y[i] = from_f64<O>(acc[i] * scale);
+  *sq = squares(y, *sq);
+}
+
+template <typename T, typename O>
+__device__ __forceinline__ O fold_one(const Sources& src, int nsrc, size_t e, double scale, double* sq) {
+  double acc = to_f64(((const T*)src.p[0])[e]);
+  for (int s = 1; s < nsrc; ++s) acc += to_f64(((const T*)src.p[s])[e]);
+  const O y = from_f64<O>(acc * scale);
+  *sq = fma(to_f64(y), to_f64(y), *sq);
+  return y;
+}
+
+// Elements [e0, e1), a vector per thread; the host gives it a block per tile
+// (a grid that loops over tiles streams 5-13% slower) but for the smallest
+// calls, which one block finishes.
+template <typename T, typename O, int NS, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void k_grad_fold(O* out, Sources src, int nsrc, size_t e0, size_t e1,
+                                                     double scale, double* parts, int held) {
+  constexpr int W = kPair<T, O>;
+  double sq = 0.0;
+  for (size_t e = e0 + ((size_t)blockIdx.x * BLOCK + threadIdx.x) * W; e < e1; e += (size_t)gridDim.x * BLOCK * W) {
+    if (e + W <= e1) {
+      O y[W];
+      fold<T, O, NS>(y, src, nsrc, e, scale, &sq);
+      store(out + e, y);
+    } else {
+      for (size_t i = e; i < e1; ++i) out[i] = fold_one<T, O>(src, nsrc, i, scale, &sq);
+    }
+  }
+  if (parts) keep<BLOCK>(parts, held, sq);
+}
+
+// The burst form of pgk_reduce_multi (pgk_reduce.hip) for gradients: every
+// thread folds TILES vectors, reads only, and stores them at the end, so the
+// chip reads and then writes.  6.5 TB/s against 5.9 for 8 sources x 64 MiB of
+// equal types; it does not pay below 5 sources, nor where the output is wider
+// (5.3 against 6.4).
+constexpr int kBurstBlock = 256;
+template <typename T, int NS, int TILES>
+__global__ __launch_bounds__(kBurstBlock) void k_grad_fold_burst(T* out, Sources src, size_t e0, size_t e1,
+                                                                 double scale, double* parts, int held) {
+  constexpr int W = kWidth<T>;
+  const size_t base = e0 + ((size_t)blockIdx.x * (kBurstBlock * TILES) + threadIdx.x) * W;
+  double sq = 0.0;
+  T y[TILES][W];
+#pragma unroll
+  for (int u = 0; u < TILES; ++u) {
+    const size_t e = base + (size_t)u * (kBurstBlock * W);
+    if (e < e1) fold<T, T, NS>(y[u], src, NS, e, scale, &sq);
+  }
+  asm volatile("" ::: "memory");                  // no store is scheduled among the loads
+#pragma unroll
+  for (int u = 0; u < TILES; ++u) {
+    const size_t e = base + (size_t)u * (kBurstBlock * W);
+    if (e < e1) store(out + e, y[u]);
+  }
+  if (parts) keep<kBurstBlock>(parts, held, sq);
 }
 
 // ---- host side ---------------------------------------------------------------------
@@ -314,91 +401,170 @@ int launched(const char* what) {
   return 0;
 }
 
-unsigned grid_for(size_t tiles) {
-  size_t g = (size_t)pgk_cu_count() * 8;
-  if (g > (size_t)kMaxGrid) g = kMaxGrid;
-  if (tiles < g) g = tiles ? tiles : 1;
-  return (unsigned)g;
+// Adds elements [at, n) of a tensor to the list, as far as a piece and the launch's tiles go;
+// returns how many were added.
+template <typename L>
+size_t add(L& l, size_t n, size_t at, size_t tile, size_t max_tiles) {
+  const size_t room = (max_tiles - l.first[l.k]) * tile, left = n - at;
+  size_t take = left < kMaxPiece ? left : kMaxPiece;
+  if (take > room) take = room;
+  l.n[l.k] = (unsigned)take;
+  l.first[l.k + 1] = l.first[l.k] + (unsigned)((take + tile - 1) / tile);
+  ++l.k;
+  return take;
 }
 
-constexpr size_t kMaxTiles = (size_t)1 << 31;      // tile numbers are 32 bits; a launch starts no later tile
+// launch(list) for lists that cover the k tensors; set(list, place, tensor, first element) fills
+// what add() does not.
+template <typename L, typename Set, typename Launch>
+int for_lists(const size_t* ns, int k, size_t tile, size_t max_tiles, Set set, Launch launch) {
+  L l;
+  l.k = 0;
+  l.first[0] = 0;
+  for (int j = 0; j < k; ++j) {
+    for (size_t at = 0; at < ns[j];) {
+      if (l.k == L::kMost || l.first[l.k] == max_tiles) {
+        if (launch(l)) return -1;
+        l.k = 0;
+      }
+      set(l, l.k, j, at);
+      at += add(l, ns[j], at, tile, max_tiles);
+    }
+  }
+  return l.k ? launch(l) : 0;
+}
+
+int finish(const char* what, const double* work, int held, double* sumsq, hipStream_t s) {
+  hipLaunchKernelGGL(k_grad_finish, dim3(1), dim3(kFinishBlock), 0, s, work, held, sumsq);
+  return launched(what);
+}
+
+// What one block of 1024 threads reads in one go (4 vectors each); a call of that size is one launch,
+// without a second one to join the sums of several blocks.
+constexpr size_t kOneBlock = 64u << 10;
+
+template <typename T, int BLOCK, int UNROLL>
+int sumsq_shape(const void* const* grads, const size_t* ns, int k, double* sumsq, double* work, hipStream_t s) {
+  using List = ReadList<kMaxRead>;
+  const bool one = sumsq == work;
+  int held = 0;
+  const int rc = for_lists<List>(
+      ns, k, (size_t)BLOCK * UNROLL * kWidth<T>, (size_t)1 << 31,
+      [&](List& l, int at, int j, size_t e) { l.p[at] = (const T*)grads[j] + e; },
+      [&](const List& l) {
+        const unsigned tiles = l.first[l.k], grid = one ? 1 : tiles < kMaxParts ? tiles : kMaxParts;
+        hipLaunchKernelGGL((k_grad_sumsq<T, BLOCK, UNROLL>), dim3(grid), dim3(BLOCK), 0, s, l, work, held);
+        if ((int)grid > held) held = (int)grid;
+        return launched("grad_sumsq");
+      });
+  if (rc || (one && held)) return rc;
+  return finish("grad_sumsq", work, held, sumsq, s);
+}
 
 template <typename T>
 int sumsq_t(const void* const* grads, const size_t* ns, int k, double* sumsq, double* work, hipStream_t s) {
-  // how many tiles the fullest launch has: every launch takes the grid that suits it
-  size_t most = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    ReadList<kMaxRead> l;
-    unsigned grid = pass ? grid_for(most) : 0;
-    size_t tiles = 0;
-    int add = 0;
-    l.k = 0;
-    for (int j = 0; j <= k; ++j) {
-      const size_t more = j < k ? (ns[j] + kTile<T> - 1) / kTile<T> : 0;
-      if (l.k && (j == k || l.k == kMaxRead || tiles + more > kMaxTiles)) {
-        if (tiles > most) most = tiles;
-        if (pass) {
-          l.first[l.k] = (unsigned)tiles;
-          hipLaunchKernelGGL((k_grad_sumsq<T>), dim3(grid), dim3(kBlock), 0, s, l, work, add);
-          if (launched("grad_sumsq")) return -1;
-          add = 1;
-        }
-        l.k = 0;
-        tiles = 0;
-      }
-      if (!more) continue;
-      l.p[l.k] = grads[j];
-      l.n[l.k] = ns[j];
-      l.first[l.k++] = (unsigned)tiles;
-      tiles += more;
-    }
-    if (pass) {
-      hipLaunchKernelGGL(k_grad_finish, dim3(1), dim3(1024), 0, s, work, add ? (int)grid : 0, sumsq);
-      return launched("grad_sumsq");
-    }
-  }
-  return 0;
+  size_t tiles = 0;
+  for (int j = 0; j < k && tiles <= 2; ++j) tiles += (ns[j] * sizeof(T) + kOneBlock - 1) / kOneBlock;
+  if (tiles <= 2) return sumsq_shape<T, 1024, 4>(grads, ns, k, sumsq, sumsq, s);
+  return sumsq_shape<T, 256, 4>(grads, ns, k, sumsq, work, s);
 }
 
 template <typename T, typename O>
 int clip_t(void* const* outs, const void* const* grads, const size_t* ns, int k, const double* sumsq, int nsum,
            double scale, double max_norm, double* norm, hipStream_t s) {
-  CopyList<kMaxCopy> l;
-  size_t tiles = 0;
+  using List = CopyList<kMaxCopy>;
   bool any = false;
-  l.k = 0;
-  for (int j = 0; j <= k; ++j) {
-    const size_t more = j < k ? (ns[j] + kTile<T> - 1) / kTile<T> : 0;
-    // a launch without tensors still writes the norm
-    if ((l.k && (j == k || l.k == kMaxCopy || tiles + more > kMaxTiles)) || (j == k && !any)) {
-      l.first[l.k] = (unsigned)tiles;
-      hipLaunchKernelGGL((k_grad_clip<T, O>), dim3(grid_for(tiles)), dim3(kBlock), 0, s, l, sumsq, nsum, scale,
-                         max_norm, any ? nullptr : norm);
-      if (launched("grad_clip")) return -1;
-      any = true;
-      l.k = 0;
-      tiles = 0;
-    }
-    if (!more) continue;
-    l.p[l.k] = grads[j];
-    l.out[l.k] = outs[j];
-    l.n[l.k] = ns[j];
-    l.first[l.k++] = (unsigned)tiles;
-    tiles += more;
-  }
-  return 0;
+  auto launch = [&](const List& l) {
+    const unsigned tiles = l.first[l.k];
+    hipLaunchKernelGGL((k_grad_clip<T, O>), dim3(tiles ? tiles : 1), dim3(kClipBlock), 0, s, l, sumsq, nsum, scale,
+                       max_norm, any ? nullptr : norm);
+    any = true;
+    return launched("grad_clip");
+  };
+  // the dispatch packet counts work-items in 32 bits: at most 2^21 blocks of 2^10
+  const int rc = for_lists<List>(
+      ns, k, (size_t)kClipBlock * kPair<T, O>, (size_t)1 << 21,
+      [&](List& l, int at, int j, size_t e) {
+        l.p[at] = (const T*)grads[j] + e;
+        l.out[at] = (O*)outs[j] + e;
+      },
+      launch);
+  if (rc || any || !norm) return rc;
+  List none;
+  none.k = 0;
+  none.first[0] = 0;
+  return launch(none);
+}
+
+template <typename T, typename O, int NS>
+void fold_launch(O* out, const Sources& src, int nsrc, size_t e0, size_t e1, double scale, double* parts, int held,
+                 unsigned grid, bool one, hipStream_t s) {
+  if (one)
+    hipLaunchKernelGGL((k_grad_fold<T, O, NS, 1024>), dim3(1), dim3(1024), 0, s, out, src, nsrc, e0, e1, scale, parts,
+                       held);
+  else
+    hipLaunchKernelGGL((k_grad_fold<T, O, NS, 512>), dim3(grid), dim3(512), 0, s, out, src, nsrc, e0, e1, scale,
+                       parts, held);
+}
+
+template <typename T, int NS>
+void burst_launch(T* out, const Sources& src, size_t e0, size_t e1, double scale, double* parts, int held,
+                  unsigned grid, int tiles, hipStream_t s) {
+  if (tiles == 32)
+    hipLaunchKernelGGL((k_grad_fold_burst<T, NS, 32>), dim3(grid), dim3(kBurstBlock), 0, s, out, src, e0, e1, scale,
+                       parts, held);
+  else
+    hipLaunchKernelGGL((k_grad_fold_burst<T, NS, 16>), dim3(grid), dim3(kBurstBlock), 0, s, out, src, e0, e1, scale,
+                       parts, held);
 }
 
 template <typename T, typename O>
 int fold_t(void* out, const Sources& src, int nsrc, size_t n, double scale, double* sumsq, double* work,
            hipStream_t s) {
-  const unsigned grid = grid_for((n + kBlock * kWidth<T> - 1) / (kBlock * kWidth<T>));
-  hipLaunchKernelGGL((k_grad_fold<T, O>), dim3(grid), dim3(kBlock), 0, s, (O*)out, src, nsrc, n, scale,
-                     sumsq ? work : nullptr);
-  if (launched("grad_fold")) return -1;
-  if (!sumsq) return 0;
-  hipLaunchKernelGGL(k_grad_finish, dim3(1), dim3(1024), 0, s, work, (int)grid, sumsq);
-  return launched("grad_fold");
+  O* o = (O*)out;
+  const bool one = n * (nsrc * sizeof(T) + sizeof(O)) <= kOneBlock;
+  double* parts = !sumsq ? nullptr : one && n ? sumsq : work;
+  size_t e0 = 0;
+  int held = 0;
+  auto ran = [&](unsigned grid, size_t e1) {
+    if ((int)grid > held) held = (int)grid;
+    e0 = e1;
+    return launched("grad_fold");
+  };
+  // the launches of the burst form hold what the waves' registers hold: 512 blocks (two per CU) of 32
+  // vectors per thread, then one of 512 to 1023 blocks of 16; what is left, under 32 MiB per source,
+  // goes a vector per thread
+  if constexpr (std::is_same_v<T, O>) {
+    constexpr size_t kHalf = (size_t)512 * kBurstBlock * 16 * kWidth<T>;      // 32 MiB per source
+    while (nsrc >= 5 && nsrc <= 8 && n - e0 >= kHalf) {
+      const int tiles = n - e0 >= 2 * kHalf ? 32 : 16;
+      const size_t per = (size_t)kBurstBlock * tiles * kWidth<T>;
+      const size_t take = tiles == 32 ? 2 * kHalf : (n - e0) / kWidth<T> * kWidth<T>;
+      const unsigned grid = (unsigned)((take + per - 1) / per);
+      switch (nsrc) {
+        case 5: burst_launch<T, 5>(o, src, e0, e0 + take, scale, parts, held, grid, tiles, s); break;
+        case 6: burst_launch<T, 6>(o, src, e0, e0 + take, scale, parts, held, grid, tiles, s); break;
+        case 7: burst_launch<T, 7>(o, src, e0, e0 + take, scale, parts, held, grid, tiles, s); break;
+        default: burst_launch<T, 8>(o, src, e0, e0 + take, scale, parts, held, grid, tiles, s);
+      }
+      if (ran(grid, e0 + take)) return -1;
+    }
+  }
+  while (e0 < n) {
+    constexpr size_t per = (size_t)512 * kPair<T, O>;
+    const size_t left = n - e0, take = one || left < per * kMaxParts ? left : per * kMaxParts;
+    const unsigned grid = one ? 1 : (unsigned)((take + per - 1) / per);
+    switch (nsrc) {
+#define PGK_FOLD_CASE(K) \
+      case K: fold_launch<T, O, K>(o, src, nsrc, e0, e0 + take, scale, parts, held, grid, one, s); break;
+      PGK_FOLD_CASE(1) PGK_FOLD_CASE(2) PGK_FOLD_CASE(3) PGK_FOLD_CASE(4)
+      PGK_FOLD_CASE(5) PGK_FOLD_CASE(6) PGK_FOLD_CASE(7)
+#undef PGK_FOLD_CASE
+      default: fold_launch<T, O, kMaxUnrolled>(o, src, nsrc, e0, e0 + take, scale, parts, held, grid, one, s);
+    }
+    if (ran(grid, e0 + take)) return -1;
+  }
+  return parts && parts != sumsq ? finish("grad_fold", work, held, sumsq, s) : 0;
 }
 
 // f(type of the gradients, type of the output) for the pairs check_types lets through.
