@@ -54,6 +54,26 @@ __device__ __forceinline__ void store(T* p, const T (&x)[N]) {
   __builtin_nontemporal_store(v, reinterpret_cast<VU*>(p));
 }
 
+// W elements packed into 16 bytes of registers, which an array of 16-bit
+// elements is not while it waits.
+template <typename T, int W>
+struct Held {
+  typedef uint32_t Words __attribute__((ext_vector_type(4)));
+  Words w;
+  __device__ __forceinline__ void put(const T (&y)[W]) {
+    typedef T V __attribute__((ext_vector_type(W)));
+    V v;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = y[i];
+    w = __builtin_bit_cast(Words, v);
+    asm("" : "+v"(w));
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    typedef Words WU __attribute__((aligned(2)));
+    __builtin_nontemporal_store(w, reinterpret_cast<WU*>(p));
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ double to_f64(T x) {
   if constexpr (sizeof(T) == 2) return (double)(float)x;
@@ -80,8 +100,9 @@ __device__ __forceinline__ O from_f64(double x) {
 // captured graph holds them.  4 KiB of kernel arguments (the runtime adds its
 // own) bound the number.  A tile is what a block takes at a time; every tensor
 // starts a tile.  A tensor of more than 2^31 elements is listed in pieces.
-constexpr int kMaxRead = 250;                     // tensors per launch, read only
-constexpr int kMaxCopy = 160;                     // tensors per launch, read and written
+constexpr int kMaxRead = 234;                     // tensors per launch, read only
+constexpr int kMaxCopy = 149;                     // tensors per launch, read and written
+constexpr int kBuckets = 128;
 constexpr size_t kMaxPiece = (size_t)1 << 31;
 constexpr int kMaxParts = PGK_GRAD_WORK_BYTES / 8;   // partial sums that the workspace holds
 
@@ -92,6 +113,8 @@ struct ReadList {
   unsigned n[K];
   unsigned first[K + 1];                          // tile at which each tensor starts
   int k;
+  int shift;                                      // bucket of a tile: t >> shift
+  unsigned where[kBuckets / 2];                   // per bucket: first and last tensor in it, 8 bits each
 };
 
 template <int K>
@@ -102,12 +125,18 @@ struct CopyList {
   unsigned n[K];
   unsigned first[K + 1];
   int k;
+  int shift;
+  unsigned where[kBuckets / 2];
 };
 
-// The tensor that tile t lies in.
+// The tensor that tile t lies in.  A search over all of them, six loads one
+// behind the other for 51 tensors, adds a quarter to a launch of one tile per
+// block (319 against 257 us for 1.6 GB); the bucket of a tile leaves none or
+// one of them in most places.
 template <typename L>
 __device__ __forceinline__ int find(const L& l, unsigned t) {
-  int lo = 0, hi = l.k - 1;
+  const unsigned b = t >> l.shift, pair = l.where[b >> 1] >> (16 * (b & 1));
+  int lo = pair & 255, hi = (pair >> 8) & 255;
   while (lo < hi) {
     const int m = (lo + hi + 1) >> 1;
     if (l.first[m] <= t) lo = m; else hi = m - 1;
@@ -202,7 +231,7 @@ __global__ __launch_bounds__(kFinishBlock) void k_grad_finish(const double* part
 
 // ---- clip --------------------------------------------------------------------------
 
-// c, and the norm it is formed from.  Every wave forms the same bits.
+// c, and the norm it is formed from, in every lane of a wave.
 __device__ __forceinline__ double coefficient(const double* sumsq, int nsum, double scale, double max_norm,
                                               double* norm) {
   double s = 0.0;
@@ -232,26 +261,39 @@ __device__ __forceinline__ O scaled(T x, double c) {
 constexpr int kClipBlock = 1024;
 template <typename T, typename O> constexpr int kPair = sizeof(T) > sizeof(O) ? kWidth<T> : kWidth<O>;
 
+// One wave of a block forms c, the others wait for it and for their loads: all
+// sixteen of them doing the 64-bit root and quotient would cost more than the
+// stream takes.
 template <typename T, typename O>
 __global__ __launch_bounds__(kClipBlock) void k_grad_clip(CopyList<kMaxCopy> l, const double* sumsq, int nsum,
                                                           double scale, double max_norm, double* norm) {
   constexpr int W = kPair<T, O>;
   constexpr unsigned kTile = kClipBlock * W;
-  double nrm;
-  if (l.first[l.k] == 0) {                         // no elements: the norm alone
-    coefficient(sumsq, nsum, scale, max_norm, &nrm);
-    if (threadIdx.x == 0) *norm = nrm;
-    return;
+  __shared__ double shared_c;
+  unsigned left = 0;                               // no elements: the norm alone
+  const T* p = nullptr;
+  O* o = nullptr;
+  if (l.first[l.k]) {
+    const int j = find(l, blockIdx.x);
+    const unsigned at = (blockIdx.x - l.first[j]) * kTile;
+    left = l.n[j] - at;
+    p = (const T*)l.p[j] + at;
+    o = (O*)l.out[j] + at;
   }
-  const int j = find(l, blockIdx.x);
-  const unsigned at = (blockIdx.x - l.first[j]) * kTile, left = l.n[j] - at, e = threadIdx.x * W;
-  const T* p = (const T*)l.p[j] + at;
-  O* o = (O*)l.out[j] + at;
-  T x[W];
+  const unsigned e = threadIdx.x * W;
   const bool whole = e + W <= left;
+  T x[W];
   if (whole) load(x, p + e);                       // on its way while c is formed
-  const double c = coefficient(sumsq, nsum, scale, max_norm, &nrm);
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = nrm;
+  if (threadIdx.x < 64) {
+    double nrm;
+    const double c = coefficient(sumsq, nsum, scale, max_norm, &nrm);
+    if (threadIdx.x == 0) {
+      shared_c = c;
+      if (norm && blockIdx.x == 0) *norm = nrm;
+    }
+  }
+  __syncthreads();
+  const double c = shared_c;
   if (whole) {
     O y[W];
 #pragma unroll
@@ -336,17 +378,21 @@ __global__ __launch_bounds__(kBurstBlock) void k_grad_fold_burst(T* out, Sources
   constexpr int W = kWidth<T>;
   const size_t base = e0 + ((size_t)blockIdx.x * (kBurstBlock * TILES) + threadIdx.x) * W;
   double sq = 0.0;
-  T y[TILES][W];
+  Held<T, W> held_y[TILES];                       // 16 bytes each: 128 registers for 32
 #pragma unroll
   for (int u = 0; u < TILES; ++u) {
     const size_t e = base + (size_t)u * (kBurstBlock * W);
-    if (e < e1) fold<T, T, NS>(y[u], src, NS, e, scale, &sq);
+    if (e < e1) {
+      T y[W];
+      fold<T, T, NS>(y, src, NS, e, scale, &sq);
+      held_y[u].put(y);
+    }
   }
   asm volatile("" ::: "memory");                  // no store is scheduled among the loads
 #pragma unroll
   for (int u = 0; u < TILES; ++u) {
     const size_t e = base + (size_t)u * (kBurstBlock * W);
-    if (e < e1) store(out + e, y[u]);
+    if (e < e1) held_y[u].store(out + e);
   }
   if (parts) keep<kBurstBlock>(parts, held, sq);
 }
@@ -414,6 +460,27 @@ size_t add(L& l, size_t n, size_t at, size_t tile, size_t max_tiles) {
   return take;
 }
 
+// Fills the buckets of a list that is complete.
+template <typename L>
+void index(L& l) {
+  static_assert(L::kMost <= 256, "tensor numbers in 8 bits");
+  const unsigned tiles = l.first[l.k];
+  l.shift = 0;
+  while (tiles && (tiles - 1) >> l.shift >= (unsigned)kBuckets) ++l.shift;
+  int lo = 0;
+  for (unsigned b = 0; b < (unsigned)kBuckets; ++b) {
+    const size_t t0 = (size_t)b << l.shift, t1 = t0 + ((size_t)1 << l.shift);   // the bucket's tiles
+    unsigned pair = 0;
+    if (t0 < tiles) {
+      while (l.first[lo + 1] <= t0) ++lo;
+      int hi = lo;
+      while (hi + 1 < l.k && l.first[hi + 1] < t1) ++hi;
+      pair = (unsigned)lo | (unsigned)hi << 8;
+    }
+    l.where[b >> 1] = b & 1 ? l.where[b >> 1] | pair << 16 : pair;
+  }
+}
+
 // launch(list) for lists that cover the k tensors; set(list, place, tensor, first element) fills
 // what add() does not.
 template <typename L, typename Set, typename Launch>
@@ -424,6 +491,7 @@ int for_lists(const size_t* ns, int k, size_t tile, size_t max_tiles, Set set, L
   for (int j = 0; j < k; ++j) {
     for (size_t at = 0; at < ns[j];) {
       if (l.k == L::kMost || l.first[l.k] == max_tiles) {
+        index(l);
         if (launch(l)) return -1;
         l.k = 0;
       }
@@ -431,7 +499,9 @@ int for_lists(const size_t* ns, int k, size_t tile, size_t max_tiles, Set set, L
       at += add(l, ns[j], at, tile, max_tiles);
     }
   }
-  return l.k ? launch(l) : 0;
+  if (!l.k) return 0;
+  index(l);
+  return launch(l);
 }
 
 int finish(const char* what, const double* work, int held, double* sumsq, hipStream_t s) {
