@@ -30,16 +30,19 @@ namespace {
 
 // N elements at any element's address, up to 16 bytes: gfx950 loads and stores
 // them at every alignment, so a tensor may start at any element of a bucket.
-// Non-temporal (nothing here is read twice by one launch): a read-only pass over
-// 1.3 GB runs at 7.0 TB/s against 6.2 with the default policy, a scaled copy of
-// 1.07 GB at 6.4 against 5.85.
+// Non-temporal but for one place (nothing here is read twice by one launch): a
+// read-only pass over 1.3 GB runs at 7.0 TB/s against 6.2 with the default policy,
+// a scaled copy of 1.07 GB at 6.4 against 5.85.
 template <typename T> constexpr int kWidth = 16 / (int)sizeof(T);
 
-template <typename T, int N>
+template <bool NT = true, typename T, int N>
 __device__ __forceinline__ void load(T (&x)[N], const T* p) {
   typedef T V __attribute__((ext_vector_type(N)));
   typedef V VU __attribute__((aligned(sizeof(T))));
-  const V v = __builtin_nontemporal_load(reinterpret_cast<const VU*>(p));
+  const VU* q = reinterpret_cast<const VU*>(p);
+  V v;
+  if constexpr (NT) v = __builtin_nontemporal_load(q);
+  else v = *q;
 #pragma unroll
   for (int i = 0; i < N; ++i) x[i] = v[i];
 }
@@ -184,7 +187,10 @@ __device__ __forceinline__ double squares(const T (&x)[N], double acc) {
 
 // A stream of reads, 16 bytes x UNROLL in flight per thread; the f64 conversions
 // and products hide behind it (accumulating in 32 bits takes the same time).
-template <typename T, int BLOCK, int UNROLL>
+// NT: what does not fit the 256 MiB Infinity Cache is read past it.  What does is
+// left there for the clip that follows: both together take 33 against 39 us for
+// 75 MiB, 66 against 74 for 150 MiB, the norm alone 14.7 against 13.6 for 75 MiB.
+template <typename T, int BLOCK, int UNROLL, bool NT>
 __global__ __launch_bounds__(BLOCK) void k_grad_sumsq(ReadList<kMaxRead> l, double* parts, int held) {
   constexpr int W = kWidth<T>;
   constexpr unsigned kTile = BLOCK * UNROLL * W;
@@ -203,14 +209,14 @@ __global__ __launch_bounds__(BLOCK) void k_grad_sumsq(ReadList<kMaxRead> l, doub
     if (left >= kTile) {
       T x[UNROLL][W];
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) load(x[u], p + (u * BLOCK + threadIdx.x) * W);
+      for (int u = 0; u < UNROLL; ++u) load<NT>(x[u], p + (u * BLOCK + threadIdx.x) * W);
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) acc = squares(x[u], acc);
     } else {
       for (unsigned e = threadIdx.x * W; e < left; e += BLOCK * W) {
         if (e + W <= left) {
           T x[W];
-          load(x, p + e);
+          load<NT>(x, p + e);
           acc = squares(x, acc);
         } else {
           for (unsigned i = e; i < left; ++i) acc = fma(to_f64(p[i]), to_f64(p[i]), acc);
@@ -257,18 +263,19 @@ __device__ __forceinline__ O scaled(T x, double c) {
 // One tile per block, one vector per thread: blocks that come and go keep reads
 // and writes mixed (a grid that loops streams 10-15% slower).  A vector is 16
 // bytes of the wider type: a lane that stores two halves of 32 bytes leaves
-// every store instruction with gaps (5.4 against 6.5 TB/s).
-constexpr int kClipBlock = 1024;
+// every store instruction with gaps (5.4 against 6.5 TB/s).  Blocks of 256 threads
+// lead by 2-6% where the types are equal (f32, 368M elements: 451 us, 464 with 512
+// threads, 478 with 1024), blocks of 1024 by 4% where the output is wider.
+template <typename T, typename O> constexpr int kClipBlock = sizeof(O) > sizeof(T) ? 1024 : 256;
 template <typename T, typename O> constexpr int kPair = sizeof(T) > sizeof(O) ? kWidth<T> : kWidth<O>;
 
-// One wave of a block forms c, the others wait for it and for their loads: all
-// sixteen of them doing the 64-bit root and quotient would cost more than the
-// stream takes.
+// One wave of a block forms c while the block's loads are on their way; the others
+// wait for it rather than do the 64-bit root and quotient as well.
 template <typename T, typename O>
-__global__ __launch_bounds__(kClipBlock) void k_grad_clip(CopyList<kMaxCopy> l, const double* sumsq, int nsum,
+__global__ __launch_bounds__((kClipBlock<T, O>)) void k_grad_clip(CopyList<kMaxCopy> l, const double* sumsq, int nsum,
                                                           double scale, double max_norm, double* norm) {
   constexpr int W = kPair<T, O>;
-  constexpr unsigned kTile = kClipBlock * W;
+  constexpr unsigned kTile = kClipBlock<T, O> * W;
   __shared__ double shared_c;
   unsigned left = 0;                               // no elements: the norm alone
   const T* p = nullptr;
@@ -346,15 +353,19 @@ __device__ __forceinline__ O fold_one(const Sources& src, int nsrc, size_t e, do
   return y;
 }
 
-// Elements [e0, e1), a vector per thread; the host gives it a block per tile
-// (a grid that loops over tiles streams 5-13% slower) but for the smallest
-// calls, which one block finishes.
-template <typename T, typename O, int NS, int BLOCK>
-__global__ __launch_bounds__(BLOCK) void k_grad_fold(O* out, Sources src, int nsrc, size_t e0, size_t e1,
-                                                     double scale, double* parts, int held) {
+// Elements [e0, e1), a vector per thread at a time, in a grid of at most as many
+// blocks as the workspace holds sums of.  Blocks of 1024 threads lose least by
+// that: 75.6 us for 3 f32 sources of 30M elements (256 threads 83, two launches
+// of 512 threads 79), 95.8 us for 4 f16 sources of 50M to f32 (105, 98); fetching
+// the next vectors ahead makes it slower.
+constexpr int kFoldBlock = 1024;
+template <typename T, typename O, int NS>
+__global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, int nsrc, size_t e0, size_t e1,
+                                                          double scale, double* parts, int held) {
   constexpr int W = kPair<T, O>;
   double sq = 0.0;
-  for (size_t e = e0 + ((size_t)blockIdx.x * BLOCK + threadIdx.x) * W; e < e1; e += (size_t)gridDim.x * BLOCK * W) {
+  for (size_t e = e0 + ((size_t)blockIdx.x * kFoldBlock + threadIdx.x) * W; e < e1;
+       e += (size_t)gridDim.x * kFoldBlock * W) {
     if (e + W <= e1) {
       O y[W];
       fold<T, O, NS>(y, src, nsrc, e, scale, &sq);
@@ -363,7 +374,7 @@ __global__ __launch_bounds__(BLOCK) void k_grad_fold(O* out, Sources src, int ns
       for (size_t i = e; i < e1; ++i) out[i] = fold_one<T, O>(src, nsrc, i, scale, &sq);
     }
   }
-  if (parts) keep<BLOCK>(parts, held, sq);
+  if (parts) keep<kFoldBlock>(parts, held, sq);
 }
 
 // The burst form of pgk_reduce_multi (pgk_reduce.hip) for gradients: every
@@ -512,8 +523,9 @@ int finish(const char* what, const double* work, int held, double* sumsq, hipStr
 // What one block of 1024 threads reads in one go (4 vectors each); a call of that size is one launch,
 // without a second one to join the sums of several blocks.
 constexpr size_t kOneBlock = 64u << 10;
+constexpr size_t kInfinityCache = 256u << 20;
 
-template <typename T, int BLOCK, int UNROLL>
+template <typename T, int BLOCK, int UNROLL, bool NT>
 int sumsq_shape(const void* const* grads, const size_t* ns, int k, double* sumsq, double* work, hipStream_t s) {
   using List = ReadList<kMaxRead>;
   const bool one = sumsq == work;
@@ -523,7 +535,7 @@ int sumsq_shape(const void* const* grads, const size_t* ns, int k, double* sumsq
       [&](List& l, int at, int j, size_t e) { l.p[at] = (const T*)grads[j] + e; },
       [&](const List& l) {
         const unsigned tiles = l.first[l.k], grid = one ? 1 : tiles < kMaxParts ? tiles : kMaxParts;
-        hipLaunchKernelGGL((k_grad_sumsq<T, BLOCK, UNROLL>), dim3(grid), dim3(BLOCK), 0, s, l, work, held);
+        hipLaunchKernelGGL((k_grad_sumsq<T, BLOCK, UNROLL, NT>), dim3(grid), dim3(BLOCK), 0, s, l, work, held);
         if ((int)grid > held) held = (int)grid;
         return launched("grad_sumsq");
       });
@@ -533,10 +545,14 @@ int sumsq_shape(const void* const* grads, const size_t* ns, int k, double* sumsq
 
 template <typename T>
 int sumsq_t(const void* const* grads, const size_t* ns, int k, double* sumsq, double* work, hipStream_t s) {
-  size_t tiles = 0;
-  for (int j = 0; j < k && tiles <= 2; ++j) tiles += (ns[j] * sizeof(T) + kOneBlock - 1) / kOneBlock;
-  if (tiles <= 2) return sumsq_shape<T, 1024, 4>(grads, ns, k, sumsq, sumsq, s);
-  return sumsq_shape<T, 256, 4>(grads, ns, k, sumsq, work, s);
+  size_t tiles = 0, bytes = 0;
+  for (int j = 0; j < k; ++j) {
+    tiles += (ns[j] * sizeof(T) + kOneBlock - 1) / kOneBlock;
+    bytes += ns[j] * sizeof(T);
+  }
+  if (tiles <= 2) return sumsq_shape<T, 1024, 4, false>(grads, ns, k, sumsq, sumsq, s);
+  if (bytes <= kInfinityCache) return sumsq_shape<T, 256, 4, false>(grads, ns, k, sumsq, work, s);
+  return sumsq_shape<T, 256, 4, true>(grads, ns, k, sumsq, work, s);
 }
 
 template <typename T, typename O>
@@ -546,14 +562,14 @@ int clip_t(void* const* outs, const void* const* grads, const size_t* ns, int k,
   bool any = false;
   auto launch = [&](const List& l) {
     const unsigned tiles = l.first[l.k];
-    hipLaunchKernelGGL((k_grad_clip<T, O>), dim3(tiles ? tiles : 1), dim3(kClipBlock), 0, s, l, sumsq, nsum, scale,
+    hipLaunchKernelGGL((k_grad_clip<T, O>), dim3(tiles ? tiles : 1), dim3(kClipBlock<T, O>), 0, s, l, sumsq, nsum, scale,
                        max_norm, any ? nullptr : norm);
     any = true;
     return launched("grad_clip");
   };
   // the dispatch packet counts work-items in 32 bits: at most 2^21 blocks of 2^10
   const int rc = for_lists<List>(
-      ns, k, (size_t)kClipBlock * kPair<T, O>, (size_t)1 << 21,
+      ns, k, (size_t)kClipBlock<T, O> * kPair<T, O>, (size_t)1 << 21,
       [&](List& l, int at, int j, size_t e) {
         l.p[at] = (const T*)grads[j] + e;
         l.out[at] = (O*)outs[j] + e;
@@ -564,17 +580,6 @@ int clip_t(void* const* outs, const void* const* grads, const size_t* ns, int k,
   none.k = 0;
   none.first[0] = 0;
   return launch(none);
-}
-
-template <typename T, typename O, int NS>
-void fold_launch(O* out, const Sources& src, int nsrc, size_t e0, size_t e1, double scale, double* parts, int held,
-                 unsigned grid, bool one, hipStream_t s) {
-  if (one)
-    hipLaunchKernelGGL((k_grad_fold<T, O, NS, 1024>), dim3(1), dim3(1024), 0, s, out, src, nsrc, e0, e1, scale, parts,
-                       held);
-  else
-    hipLaunchKernelGGL((k_grad_fold<T, O, NS, 512>), dim3(grid), dim3(512), 0, s, out, src, nsrc, e0, e1, scale,
-                       parts, held);
 }
 
 template <typename T, int NS>
@@ -620,19 +625,19 @@ int fold_t(void* out, const Sources& src, int nsrc, size_t n, double scale, doub
       if (ran(grid, e0 + take)) return -1;
     }
   }
-  while (e0 < n) {
-    constexpr size_t per = (size_t)512 * kPair<T, O>;
-    const size_t left = n - e0, take = one || left < per * kMaxParts ? left : per * kMaxParts;
-    const unsigned grid = one ? 1 : (unsigned)((take + per - 1) / per);
+  if (e0 < n) {
+    constexpr size_t per = (size_t)kFoldBlock * kPair<T, O>;
+    const size_t tiles = (n - e0 + per - 1) / per;
+    const unsigned grid = one ? 1 : tiles < (size_t)kMaxParts ? (unsigned)tiles : kMaxParts;
     switch (nsrc) {
-#define PGK_FOLD_CASE(K) \
-      case K: fold_launch<T, O, K>(o, src, nsrc, e0, e0 + take, scale, parts, held, grid, one, s); break;
-      PGK_FOLD_CASE(1) PGK_FOLD_CASE(2) PGK_FOLD_CASE(3) PGK_FOLD_CASE(4)
-      PGK_FOLD_CASE(5) PGK_FOLD_CASE(6) PGK_FOLD_CASE(7)
+#define PGK_FOLD_CASE(NS, K) \
+      K: hipLaunchKernelGGL((k_grad_fold<T, O, NS>), dim3(grid), dim3(kFoldBlock), 0, s, o, src, nsrc, e0, n, scale, \
+                            parts, held); break;
+      PGK_FOLD_CASE(1, case 1) PGK_FOLD_CASE(2, case 2) PGK_FOLD_CASE(3, case 3) PGK_FOLD_CASE(4, case 4)
+      PGK_FOLD_CASE(5, case 5) PGK_FOLD_CASE(6, case 6) PGK_FOLD_CASE(7, case 7) PGK_FOLD_CASE(kMaxUnrolled, default)
 #undef PGK_FOLD_CASE
-      default: fold_launch<T, O, kMaxUnrolled>(o, src, nsrc, e0, e0 + take, scale, parts, held, grid, one, s);
     }
-    if (ran(grid, e0 + take)) return -1;
+    if (ran(grid, n)) return -1;
   }
   return parts && parts != sumsq ? finish("grad_fold", work, held, sumsq, s) : 0;
 }
