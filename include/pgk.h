@@ -159,8 +159,8 @@ PG_API int pgk_all_reduce_staged(void *const *sendbufs, void *const *recvbufs, i
  * Tensors are contiguous, on a multiple of their element size (16-byte
  * alignment is not needed), up to 2^40 elements each; a tensor of 0 elements is
  * skipped and its pointer may be NULL.  Elements between and behind the tensors
- * are neither read nor written.  Any number of tensors: a launch holds 234 of
- * them (pgk_grad_sumsq) or 149 (pgk_grad_clip).
+ * are neither read nor written.  Any number of tensors: a launch holds 351 of
+ * them (218 in a pgk_grad_clip whose outputs do not lie as the gradients do).
  *
  * work: PGK_GRAD_WORK_BYTES of device memory, 8-byte aligned, any contents.  A
  * call uses it until it has run on its stream; calls that may overlap in time

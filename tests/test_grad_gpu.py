@@ -109,7 +109,8 @@ EDGES = [1, 2, 3, 7, 8, 9, 63, 64, 65, 255, 257, 511, 513, 1023, 1024, 1025, 204
 LISTS = {
     "none": [], "empty": [0], "empties": [0, 0, 0], "one": [1], "one-between-empties": [0, 1, 0],
     "edges": EDGES, "edges-backwards": EDGES[::-1], "one-large": [1_000_003],
-    "fills-a-launch": [5] * 180, "one-more": [5] * 181, "many": [(37 * i) % 301 for i in range(1000)],
+    "fills-a-launch": [5] * 351, "one-more": [5] * 352, "fills-with-outputs": [5] * 218, "one-more-with-outputs": [5] * 219,
+    "many": [(37 * i) % 301 for i in range(1000)],
     "large-behind-many": [3] * 400 + [300_001], "large-before-many": [300_001] + [3] * 400,
 }
 
