@@ -179,6 +179,22 @@ PG_API int pgx_sim_run(int world, int coll, void *const *sendbufs, void *const *
  * of the hot path is measured on. */
 PG_API int pgx_reduce_host(void *dst, const void *src, size_t n, int datatype, int op, size_t chunk_bytes);
 
+/* No counterpart in the reference.  Clip gradients that are spread over the ranks
+ * by their global norm: pgk_grad_sumsq over this rank's k tensors, the ranks'
+ * sums added up (one pg_all_reduce of two doubles), pgk_grad_clip by the result.
+ * include/pgk.h has the types, the formula and what tensors have to be like; here
+ * they are device memory of the handle's device, complete or produced on the null
+ * stream (as the device buffers of every pg_* call).  Each rank has its own
+ * tensors (its reduce-scatter shard, its pipeline stage; none at all with k = 0):
+ * a tensor that several ranks hold counts on each of them.  scale and max_norm
+ * are the same on every rank.  *norm (host, may be NULL): the norm, the same on
+ * every rank.  Synchronous.  A rank whose arguments are refused makes the call
+ * return -1 on every rank, with every tensor as it was.  world_size == 1 needs no
+ * exchange; PG_TRANSPORT_LOOPBACK has no all-reduce and returns -1.
+ * pg_get_stats describes the all-reduce inside. */
+PG_API int pg_grad_clip(void *const *outs, int out_dt, const void *const *grads, int dt, const size_t *ns, int k,
+                        double scale, double max_norm, double *norm, void *pg_handle);
+
 /* Measurements of the last collective on this handle. */
 struct pg_stats {
   double wall_us;        /* host wall time of the call                      */

@@ -325,6 +325,7 @@ void pg_impl_destroy(struct pg *pg) {
   if (im->dsrc) hipFree(im->dsrc);
   if (im->dout) hipFree(im->dout);
   if (im->ebuf) hipFree(im->ebuf);
+  if (im->gwork) hipFree(im->gwork);
   free(im->steps);
   free(im);
   pg->impl = NULL;

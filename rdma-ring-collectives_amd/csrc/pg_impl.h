@@ -83,6 +83,7 @@ struct pg_impl {
   void *dsrc;      size_t dsrc_cap;   /* device copy of a host sendbuf        */
   void *dout;      size_t dout_cap;   /* device result / full buffer          */
   void *ebuf;      size_t ebuf_cap;   /* eager one-shot gather area (pg_eager.c) */
+  void *gwork;     size_t gwork_cap;  /* workspace and sum of pg_grad_clip (pg_grad.c) */
   int eager_oneshot;          /* PG_EAGER_ONESHOT, default 1                  */
   int rings;                  /* PG_RINGS: 1 .. 4, default 2, pg_ext.h         */
   int algo;                   /* PG_ALGO: PG_ALGO_RING / PG_ALGO_DIRECT (P2P transports) */

@@ -579,9 +579,13 @@ int finish(const char* what, const double* work, int held, double* sumsq, hipStr
   return launched(what);
 }
 
-// What one block of 1024 threads reads in one go (4 vectors each); a call of that size is one launch,
-// without a second one to join the sums of several blocks.
-constexpr size_t kOneBlock = 64u << 10;
+// Up to here one block of 1024 threads does a call in one launch, without a second
+// one to join the sums of several blocks: 256 KiB of f32 in 5.9 us against 7.6 (512 KiB:
+// 8.6 against 7.6), 2 sources of 80 KB folded in 6.3 us against 7.2.  Joining them in
+// the same launch, by the block that finishes last, loses from 128 blocks on: their
+// counter is one address across eight dies (1024 blocks 37 us, two launches 10.3).
+constexpr size_t kOneBlock = 256u << 10;
+constexpr size_t kOneBlockTile = 64u << 10;       // what it takes at a time, 4 vectors per thread
 constexpr size_t kInfinityCache = 256u << 20;
 
 // The blocks of a norm launch: 3 of 256 threads per CU (4 for f64) lead, and leave
@@ -610,10 +614,10 @@ template <typename T>
 int sumsq_t(const void* const* grads, const size_t* ns, int k, double* sumsq, double* work, hipStream_t s) {
   size_t tiles = 0, bytes = 0;
   for (int j = 0; j < k; ++j) {
-    tiles += (ns[j] * sizeof(T) + kOneBlock - 1) / kOneBlock;
+    tiles += (ns[j] * sizeof(T) + kOneBlockTile - 1) / kOneBlockTile;
     bytes += ns[j] * sizeof(T);
   }
-  if (tiles <= 2) return sumsq_shape<T, 1024, 4, false>(grads, ns, k, sumsq, sumsq, s);
+  if (tiles <= kOneBlock / kOneBlockTile) return sumsq_shape<T, 1024, 4, false>(grads, ns, k, sumsq, sumsq, s);
   if (bytes <= kInfinityCache) return sumsq_shape<T, 256, 4, false>(grads, ns, k, sumsq, work, s);
   return sumsq_shape<T, 256, 4, true>(grads, ns, k, sumsq, work, s);
 }
@@ -730,14 +734,11 @@ int pgk_grad_sumsq(const void* const* grads, const size_t* ns, int k, int dt, do
   });
 }
 
-int pgk_grad_clip(void* const* outs, int out_dt, const void* const* grads, int dt, const size_t* ns, int k,
-                  const double* sumsq, int nsum, double scale, double max_norm, double* norm, void* stream) {
+int pgk_grad_clip_check(void* const* outs, int out_dt, const void* const* grads, int dt, const size_t* ns, int k,
+                        double scale, double max_norm) {
   const char* what = "grad_clip";
   if (!check_types(what, dt, out_dt) || !check_list(what, grads, ns, k, elem_size(dt)) ||
-      !check_list(what, (const void* const*)outs, ns, k, elem_size(out_dt)) ||
-      !check_sums(what, sumsq, "sumsq") || (norm && !check_sums(what, norm, "norm"))) return -1;
-  if (nsum < 1) { set_err("pgk: %s: %d partial sums", what, nsum); return -1; }
-  if (norm && overlap(norm, 8, sumsq, (size_t)nsum * 8)) { set_err("pgk: %s: norm lies in sumsq", what); return -1; }
+      !check_list(what, (const void* const*)outs, ns, k, elem_size(out_dt))) return -1;
   if (!isfinite(scale)) { set_err("pgk: %s: scale %g", what, scale); return -1; }
   if (!(max_norm >= 0)) { set_err("pgk: %s: max_norm %g", what, max_norm); return -1; }
   for (int j = 0; j < k; ++j)
@@ -746,6 +747,16 @@ int pgk_grad_clip(void* const* outs, int out_dt, const void* const* grads, int d
       set_err("pgk: %s: output %d overlaps its gradient at a different address", what, j);
       return -1;
     }
+  return 0;
+}
+
+int pgk_grad_clip(void* const* outs, int out_dt, const void* const* grads, int dt, const size_t* ns, int k,
+                  const double* sumsq, int nsum, double scale, double max_norm, double* norm, void* stream) {
+  const char* what = "grad_clip";
+  if (pgk_grad_clip_check(outs, out_dt, grads, dt, ns, k, scale, max_norm) || !check_sums(what, sumsq, "sumsq") ||
+      (norm && !check_sums(what, norm, "norm"))) return -1;
+  if (nsum < 1) { set_err("pgk: %s: %d partial sums", what, nsum); return -1; }
+  if (norm && overlap(norm, 8, sumsq, (size_t)nsum * 8)) { set_err("pgk: %s: norm lies in sumsq", what); return -1; }
   return with_types(dt, out_dt, [&](auto* t, auto* o) {
     return clip_t<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>>(
         outs, grads, ns, k, sumsq, nsum, scale, max_norm, norm, (hipStream_t)stream);

@@ -436,7 +436,7 @@ int cu_count() {
 
 }  // namespace
 
-int pgk_cu_count() { return cu_count(); }
+int pgk_cu_count(void) { return cu_count(); }
 
 namespace {
 

@@ -108,6 +108,8 @@ _SIGS = {
     "pgx_xgmi_mode": (_I, [_VP, ctypes.POINTER(_I), ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
     "pg_connect_local": (_I, [_I, _I, _I, ctypes.POINTER(_VP)]),
     "pgx_sim_run": (_I, [_I, _I, ctypes.POINTER(_VP), ctypes.POINTER(_VP), _I, _I, _I, _SZ, _SZ, _I, _I]),
+    "pg_grad_clip": (_I, [ctypes.POINTER(_VP), _I, ctypes.POINTER(_VP), _I, ctypes.POINTER(_SZ), _I, ctypes.c_double,
+                          ctypes.c_double, ctypes.POINTER(ctypes.c_double), _VP]),
     "pg_get_stats": (_I, [_VP, ctypes.POINTER(PgStats)]),
     "pgx_reduce_host": (_I, [_VP, _CVP, _SZ, _I, _I, _SZ]),
     "pg_last_error": (ctypes.c_char_p, []),
@@ -246,6 +248,17 @@ def plan_coalesce(steps, es):
     if k < 0:
         raise ValueError("pg_plan_coalesce: bad arguments")
     return [{name: getattr(out[i], name) for name, _ in PgRedRange._fields_} for i in range(k)]
+
+
+def tensor_list(tensors):
+    """(pointers, element counts, number) of contiguous torch tensors, as the
+    pgk_grad_* calls take them.  It holds no reference: keep the tensors."""
+    for i, t in enumerate(tensors):
+        if not t.is_contiguous():
+            raise ValueError(f"tensor {i} is not contiguous")
+    k = len(tensors)
+    pointers = (ctypes.c_void_p * max(k, 1))(*[t.data_ptr() or None for t in tensors])
+    return pointers, (ctypes.c_size_t * max(k, 1))(*[t.numel() for t in tensors]), k
 
 
 def head(handle) -> PgHead:

@@ -116,3 +116,20 @@ def test_overlaps(lib):
 def test_nothing_to_fold(lib):
     """n = 0 without a sum asked for is a no-op that needs no buffers."""
     assert lib.pgk_grad_fold(None, F32, None, 2, 0, F32, 1.0, None, None, None) == 0
+
+
+def test_tensor_list():
+    """pgamd.tensor_list: what the calls take, from contiguous torch tensors."""
+    import torch
+    ts = [torch.zeros(5), torch.zeros(0), torch.zeros(2, 3, dtype=torch.bfloat16)]
+    p, n, k = pgamd.tensor_list(ts)
+    assert k == 3 and list(n) == [5, 0, 6]
+    assert p[0] == ts[0].data_ptr() and p[2] == ts[2].data_ptr()
+    assert pgamd.tensor_list([])[2] == 0
+    with pytest.raises(ValueError, match="tensor 1"):
+        pgamd.tensor_list([torch.zeros(4), torch.zeros(4, 4).t()])
+
+
+def test_group_call_needs_a_handle(lib):
+    assert lib.pg_grad_clip(None, F32, None, F32, None, 0, 1.0, 1.0, None, None) == -1
+    assert b"NULL handle" in lib.pg_last_error()
