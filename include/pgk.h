@@ -173,7 +173,7 @@ PG_API int pgk_all_reduce_staged(void *const *sendbufs, void *const *recvbufs, i
 #define PGK_DT_BF16 4
 #define PGK_GRAD_WORK_BYTES 65536
 
-/* *sumsq (device) = the sum of the squares of all elements of the k tensors,
+/* *sumsq (device, outside work) = the sum of the squares of all elements of the k tensors,
  * formed and summed in 64 bits: no f32, f16 or bf16 value overflows or
  * underflows in it.  A NaN or an infinity among the gradients gives NaN or
  * infinity.  No tensors, or empty ones only: 0.  The gradient norm is its
@@ -187,16 +187,16 @@ PG_API int pgk_grad_sumsq(const void *const *grads, const size_t *ns, int k, int
  *     c = scale * min(1, max_norm / (norm + 1e-6))
  *     outs[j][i] = c * grads[j][i]     for i < ns[j], j < k
  * scale (finite) is what the gradients are multiplied by in any case: 1, the
- * 1 / world_size of a mean, the inverse of a loss scale.  max_norm >= 0;
- * infinity does not clip.  *norm (device, may be NULL) receives the norm, also
- * when k = 0.  f64 and f32 results are rounded once, from a 64-bit product;
- * f16 and bf16 ones from a 32-bit product.
+ * 1 / world_size of a mean, the inverse of a loss scale.  max_norm >= 0; with
+ * infinity nothing is clipped, c = scale.  *norm (device, may be NULL) receives
+ * the norm, also when k = 0.  Products are formed in 64 bits and rounded to the
+ * output's type (f16 and bf16 by way of f32).
  * A norm that is not finite clips as the formula says: an infinite one gives 0,
  * and NaN where the gradient is infinite; NaN gives NaN everywhere.  A caller
  * who would rather skip such a step looks at *norm first.
  * outs[j] == grads[j] (in place) is allowed when the types are equal; other
  * overlaps are not (within a pair they are refused), nor is a tensor that is
- * listed twice. */
+ * listed twice.  In place with c == 1 the gradients are left as they are. */
 PG_API int pgk_grad_clip(void *const *outs, int out_dt, const void *const *grads, int dt, const size_t *ns, int k,
                          const double *sumsq, int nsum, double scale, double max_norm, double *norm, void *stream);
 
@@ -204,10 +204,11 @@ PG_API int pgk_grad_clip(void *const *outs, int out_dt, const void *const *grads
  * srcs[nsrc-1][i]) for i < n, 1 <= nsrc <= 16, summed left to right in 64 bits
  * and rounded to the output's type at the end (f16 and bf16 by way of f32).
  * scale (finite): 1, or 1 / nsrc for the mean.
- * sumsq (device, may be NULL): the sum of the squares of out as stored, what
- * pgk_grad_sumsq over out would give up to the order of its sum, without reading
- * it again.  Without sumsq, work may be NULL.  n = 0 gives 0.  Sources may be peer GPUs' memory as in
- * pgk_reduce_multi; out may be one of them when the types are equal. */
+ * sumsq (device, outside work, may be NULL): the sum of the squares of out as
+ * stored, what pgk_grad_sumsq over out would give up to the order of its sum,
+ * without reading it again; 0 when n = 0.  Without sumsq, work may be NULL.
+ * Sources may be peer GPUs' memory as in pgk_reduce_multi; out may be one of them
+ * when the types are equal. */
 PG_API int pgk_grad_fold(void *out, int out_dt, const void *const *srcs, int nsrc, size_t n, int dt, double scale,
                          double *sumsq, void *work, void *stream);
 

@@ -30,7 +30,7 @@ namespace {
 
 // N elements at any element's address, up to 16 bytes: gfx950 loads and stores
 // them at every alignment, so a tensor may start at any element of a bucket.
-// Non-temporal but for one place (nothing here is read twice by one launch): a
+// Non-temporal but where it says otherwise (nothing here is read twice by one launch): a
 // read-only pass over 1.3 GB runs at 7.0 TB/s against 6.2 with the default policy,
 // a scaled copy of 1.07 GB at 6.4 against 5.85.
 template <typename T> constexpr int kWidth = 16 / (int)sizeof(T);
@@ -47,14 +47,15 @@ __device__ __forceinline__ void load(T (&x)[N], const T* p) {
   for (int i = 0; i < N; ++i) x[i] = v[i];
 }
 
-template <typename T, int N>
+template <bool NT = true, typename T, int N>
 __device__ __forceinline__ void store(T* p, const T (&x)[N]) {
   typedef T V __attribute__((ext_vector_type(N)));
   typedef V VU __attribute__((aligned(sizeof(T))));
   V v;
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = x[i];
-  __builtin_nontemporal_store(v, reinterpret_cast<VU*>(p));
+  if constexpr (NT) __builtin_nontemporal_store(v, reinterpret_cast<VU*>(p));
+  else *reinterpret_cast<VU*>(p) = v;
 }
 
 // W elements as they lie in memory.  What waits in registers waits like this: the
@@ -84,7 +85,7 @@ struct Raw {
   }
   __device__ __forceinline__ void store(T* p) const {
     typedef Words WU __attribute__((aligned(2)));
-    __builtin_nontemporal_store(w, reinterpret_cast<WU*>(p));
+    *reinterpret_cast<WU*>(p) = w;
   }
 };
 
@@ -290,15 +291,7 @@ __device__ __forceinline__ double coefficient(const double* sumsq, int nsum, dou
   }
   *norm = fabs(scale) * sqrt(s);
   const double c = max_norm / (*norm + 1e-6);
-  return scale * (c > 1.0 ? 1.0 : c);              // a NaN stays one
-}
-
-// What the product is formed in: 64 bits where the result keeps 24 bits or more
-// (one rounding, to the stored type), 32 bits for a 16-bit result.
-template <typename O, typename T>
-__device__ __forceinline__ O scaled(T x, double c) {
-  if constexpr (sizeof(O) == 2) return (O)((float)x * (float)c);
-  else return (O)(to_f64(x) * c);
+  return c > 1.0 || isinf(max_norm) ? scale : scale * c;   // a NaN of the norm's stays one
 }
 
 // One tile per block, one vector per thread: blocks that come and go keep reads
@@ -335,15 +328,18 @@ __global__ __launch_bounds__((kClipBlock<T, O>)) void k_grad_clip(List<OWN_OUT> 
   }
   __syncthreads();
   const double c = shared_c;
+  // in place, a step that is not clipped needs no writes
+  if constexpr (std::is_same_v<T, O>)
+    if (o == p && c == 1.0) return;
   if (whole) {
     T x[W];
     O y[W];
     raw.get(x);
 #pragma unroll
-    for (int i = 0; i < W; ++i) y[i] = scaled<O>(x[i], c);
+    for (int i = 0; i < W; ++i) y[i] = from_f64<O>(to_f64(x[i]) * c);
     store(o + e, y);
   } else {
-    for (unsigned i = e; i < left; ++i) o[i] = scaled<O>(p[i], c);
+    for (unsigned i = e; i < left; ++i) o[i] = from_f64<O>(to_f64(p[i]) * c);
   }
 }
 
@@ -400,7 +396,9 @@ __device__ __forceinline__ O fold_one(const Sources& src, int nsrc, size_t e, do
 // blocks as the workspace holds sums of.  Blocks of 1024 threads lose least by
 // that: 75.6 us for 3 f32 sources of 30M elements (256 threads 83, two launches
 // of 512 threads 79), 95.8 us for 4 f16 sources of 50M to f32 (105, 98); fetching
-// the next vectors ahead makes it slower.
+// the next vectors ahead makes it slower.  An output whose sum is wanted stays in
+// the caches, as far as it fits, for the clip that follows: 3 f32 sources of 30M
+// elements take 85 instead of 79 us, with the clip 114 instead of 120.
 constexpr int kFoldBlock = 1024;
 template <typename T, typename O, int NS>
 __global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, int nsrc, size_t e0, size_t e1,
@@ -412,7 +410,8 @@ __global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, i
     if (e + W <= e1) {
       O y[W];
       fold<T, O, NS>(y, src, nsrc, e, scale, &sq);
-      store(out + e, y);
+      if (parts) store<false>(out + e, y);
+      else store(out + e, y);
     } else {
       for (size_t i = e; i < e1; ++i) out[i] = fold_one<T, O>(src, nsrc, i, scale, &sq);
     }
@@ -424,7 +423,9 @@ __global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, i
 // thread folds TILES vectors, reads only, and stores them at the end, so the
 // chip reads and then writes.  6.5 TB/s against 5.9 for 8 sources x 64 MiB of
 // equal types; it does not pay below 5 sources, nor where the output is wider
-// (5.3 against 6.4).
+// (5.3 against 6.4).  Its stores come in one burst and cost the same with the
+// default policy, which leaves the output to what follows (with a clip 117 against
+// 122 us for 8 x 64 MiB).
 constexpr int kBurstBlock = 256;
 template <typename T, int NS, int TILES>
 __global__ __launch_bounds__(kBurstBlock) void k_grad_fold_burst(T* out, Sources src, size_t e0, size_t e1,
@@ -493,6 +494,12 @@ bool check_list(const char* what, const void* const* p, const size_t* ns, int k,
 
 bool check_sums(const char* what, const void* p, const char* name) {
   if (!p || misaligned(p, 8)) { set_err("pgk: %s: %s is NULL or not 8-byte aligned", what, name); return false; }
+  return true;
+}
+
+bool check_work(const char* what, const double* sumsq, const void* work) {
+  if (!check_sums(what, sumsq, "sumsq") || !check_sums(what, work, "work")) return false;
+  if (overlap(sumsq, 8, work, PGK_GRAD_WORK_BYTES)) { set_err("pgk: %s: sumsq lies in work", what); return false; }
   return true;
 }
 
@@ -594,15 +601,16 @@ constexpr size_t kInfinityCache = 256u << 20;
 template <typename T> constexpr int kBlocksPerCu = sizeof(T) == 8 ? 4 : 3;
 
 template <typename T, int BLOCK, int UNROLL, bool NT>
-int sumsq_shape(const void* const* grads, const size_t* ns, int k, double* sumsq, double* work, hipStream_t s) {
+int sumsq_shape(const void* const* grads, const size_t* ns, int k, double* sumsq, double* work, bool one,
+                hipStream_t s) {
   constexpr unsigned kTile = BLOCK * UNROLL * kWidth<T>;
-  const bool one = sumsq == work;
   const unsigned full = (unsigned)pgk_cu_count() * kBlocksPerCu<T>;
   const unsigned most = one ? 1 : full < (unsigned)kMaxParts ? full : kMaxParts;
+  double* const parts = one ? sumsq : work;
   int held = 0;
   const int rc = for_lists<T, T, kTile, false>(grads, nullptr, ns, k, [&](const List<false>& l) {
     const unsigned tiles = tiles_of<kTile>(l), grid = tiles < most ? tiles : most;
-    hipLaunchKernelGGL((k_grad_sumsq<T, BLOCK, UNROLL, NT>), dim3(grid), dim3(BLOCK), 0, s, l, grid, work, held);
+    hipLaunchKernelGGL((k_grad_sumsq<T, BLOCK, UNROLL, NT>), dim3(grid), dim3(BLOCK), 0, s, l, grid, parts, held);
     if ((int)grid > held) held = (int)grid;
     return launched("grad_sumsq");
   });
@@ -617,9 +625,9 @@ int sumsq_t(const void* const* grads, const size_t* ns, int k, double* sumsq, do
     tiles += (ns[j] * sizeof(T) + kOneBlockTile - 1) / kOneBlockTile;
     bytes += ns[j] * sizeof(T);
   }
-  if (tiles <= kOneBlock / kOneBlockTile) return sumsq_shape<T, 1024, 4, false>(grads, ns, k, sumsq, sumsq, s);
-  if (bytes <= kInfinityCache) return sumsq_shape<T, 256, 4, false>(grads, ns, k, sumsq, work, s);
-  return sumsq_shape<T, 256, 4, true>(grads, ns, k, sumsq, work, s);
+  if (tiles <= kOneBlock / kOneBlockTile) return sumsq_shape<T, 1024, 4, false>(grads, ns, k, sumsq, work, true, s);
+  if (bytes <= kInfinityCache) return sumsq_shape<T, 256, 4, false>(grads, ns, k, sumsq, work, false, s);
+  return sumsq_shape<T, 256, 4, true>(grads, ns, k, sumsq, work, false, s);
 }
 
 template <typename T, typename O, bool OWN_OUT>
@@ -728,7 +736,7 @@ int pgk_grad_sumsq(const void* const* grads, const size_t* ns, int k, int dt, do
                    void* stream) {
   const char* what = "grad_sumsq";
   if (!check_types(what, dt, dt) || !check_list(what, grads, ns, k, elem_size(dt)) ||
-      !check_sums(what, sumsq, "sumsq") || !check_sums(what, work, "work")) return -1;
+      !check_work(what, sumsq, work)) return -1;
   return with_types(dt, dt, [&](auto* t, auto*) {
     return sumsq_t<std::remove_pointer_t<decltype(t)>>(grads, ns, k, sumsq, (double*)work, (hipStream_t)stream);
   });
@@ -769,7 +777,7 @@ int pgk_grad_fold(void* out, int out_dt, const void* const* srcs, int nsrc, size
   if (!check_types(what, dt, out_dt)) return -1;
   if (nsrc < 1 || nsrc > kMaxSrc) { set_err("pgk: %s: nsrc %d outside 1..%d", what, nsrc, kMaxSrc); return -1; }
   if (!isfinite(scale)) { set_err("pgk: %s: scale %g", what, scale); return -1; }
-  if (sumsq && (!check_sums(what, sumsq, "sumsq") || !check_sums(what, work, "work"))) return -1;
+  if (sumsq && !check_work(what, sumsq, work)) return -1;
   const size_t es = elem_size(dt), oes = elem_size(out_dt);
   Sources src{};
   if (n) {

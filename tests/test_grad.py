@@ -85,6 +85,11 @@ def test_places_of_results(lib):
         refused(lib, lib.pgk_grad_sumsq(g, n, 1, F32, SUM, bad, None), "work")
         refused(lib, lib.pgk_grad_clip(g, F32, g, F32, n, 1, bad, 1, 1.0, 1.0, None, None), "sumsq")
         refused(lib, lib.pgk_grad_fold(BASE, F32, g, 1, 4, F32, 1.0, SUM, bad, None), "work")
+    big = (ctypes.c_double * (pgamd.PGK_GRAD_WORK_BYTES // 8))()
+    work = ctypes.addressof(big)
+    for inside in (work, work + 8, work + pgamd.PGK_GRAD_WORK_BYTES - 8):
+        refused(lib, lib.pgk_grad_sumsq(g, n, 1, F32, inside, work, None), "sumsq lies in work")
+        refused(lib, lib.pgk_grad_fold(BASE, F32, g, 1, 4, F32, 1.0, inside, work, None), "sumsq lies in work")
     refused(lib, lib.pgk_grad_clip(g, F32, g, F32, n, 1, SUM, 1, 1.0, 1.0, NORM + 4, None), "norm")
     refused(lib, lib.pgk_grad_clip(g, F32, g, F32, n, 1, SUM, 3, 1.0, 1.0, SUM + 16, None), "norm lies in sumsq")
     for nsum in (0, -1):

@@ -7,10 +7,9 @@ Tolerances.  h = finfo.eps / 2 is the half step that one rounding may be off by.
           of an f64 value within one more on either side, and the two sums of the
           reference are rounded once each: (n + 3) 2^-53, relative.
   clip    c takes a sum of nsum terms, a root, two products, a sum and a quotient:
-          within (nsum + 6) 2^-53.  f64 results add one product; f32 ones are
-          rounded once more, h = 2^-24; 16-bit ones come from c rounded to 32 bits
-          and a 32-bit product: h + 2 * 2^-24 (1 + h).  Below the smallest normal
-          number a rounding is off by half the smallest subnormal one.
+          within (nsum + 6) 2^-53.  The product adds 2^-53, its rounding to f32
+          2^-24, that to 16 bits h.  Below the smallest normal number a rounding is
+          off by half the smallest subnormal one.
   fold    the same IEEE operations in the same order: equal bits.
 """
 import ctypes
@@ -171,8 +170,8 @@ def allowed(want, out_dt, nsum):
     """How far each result may be from `want` (f64); see the head of the file."""
     f = torch.finfo(TYPES[out_dt][1])
     h, c = f.eps / 2, (nsum + 6) * U
-    step = {"f64": h, "f32": h + U, "f16": h + 2 * 2.0 ** -24 * (1 + h), "bf16": h + 2 * 2.0 ** -24 * (1 + h)}[out_dt]
-    return want.abs() * (step + c) * (1 + 2 * h) + f.smallest_normal * f.eps / 2
+    step = {"f64": U, "f32": h + U, "f16": h + 2.0 ** -24 + U, "bf16": h + 2.0 ** -24 + U}[out_dt]
+    return want.abs() * (step + c) * (1 + 2 * h) + f.smallest_normal * f.eps / 2 * (1 + 2.0 ** -8)
 
 
 @pytest.mark.parametrize("dt,out_dt", PAIRS)
@@ -229,6 +228,33 @@ def test_clip_at_the_ends_of_max_norm(gpu, lib):
     assert all(torch.equal(o, t) for o, t in zip(outs, ts))               # norm 0: nothing is clipped
     assert float(clip(lib, outs, "f32", ts, "f32", cell(1e200), 0.0, 1.0)) == 0.0
     assert all((o == 0).all() for o in outs)                              # scale = 0
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32", "f64"])
+def test_clip_of_gradients_that_exploded(gpu, lib, dt):
+    """Norms of 1e41 and more: c is below what 32 bits hold with any precision, the results are not."""
+    _, ts = bucket([5000], "f64", 55)
+    t = (ts[0] / ts[0].abs().max() * 3e38).to(TYPES[dt][1])
+    out = torch.empty_like(t)
+    s = sumsq(lib, [t], dt)
+    clip(lib, [out], dt, [t], dt, s, 1e-3, 1e-3)
+    _, c = coefficient([exact_sumsq([t])], 1e-3, 1e-3)
+    assert 0 < c < 1e-40
+    want = t.cpu().double() * c
+    assert ((out.cpu().double() - want).abs() <= allowed(want, dt, 5000)).all()
+
+
+@pytest.mark.parametrize("dt,out_dt", PAIRS)
+def test_clip_without_a_limit_keeps_what_is_not_finite_to_itself(gpu, lib, dt, out_dt):
+    """max_norm = infinity scales and no more, whatever the norm is."""
+    t = torch.ones(3000, dtype=TYPES[dt][1], device="cuda")
+    t[3], t[4] = math.inf, math.nan
+    out = torch.empty(3000, dtype=TYPES[out_dt][1], device="cuda")
+    for value in (math.inf, math.nan):
+        norm = clip(lib, [out], out_dt, [t], dt, cell(value), 0.5, math.inf)
+        assert math.isnan(float(norm)) if math.isnan(value) else float(norm) == math.inf
+        got = out.cpu().double()
+        assert got[3] == math.inf and got[4].isnan() and int((got == 0.5).sum()) == 2998
 
 
 @pytest.mark.parametrize("dt,out_dt", PAIRS)
