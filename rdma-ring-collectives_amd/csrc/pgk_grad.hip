@@ -294,30 +294,34 @@ __device__ __forceinline__ double coefficient(const double* sumsq, int nsum, dou
   return c > 1.0 || isinf(max_norm) ? scale : scale * c;   // a NaN of the norm's stays one
 }
 
-// One tile per block, one vector per thread: blocks that come and go keep reads
-// and writes mixed (a grid that loops streams 10-15% slower).  A vector is 16
-// bytes of the wider type: a lane that stores two halves of 32 bytes leaves
-// every store instruction with gaps (5.4 against 6.5 TB/s).  Blocks of 256 threads
-// lead by 2-6% where the types are equal (f32, 368M elements: 451 us, 464 with 512
-// threads, 478 with 1024), blocks of 1024 by 4% where the output is wider.
-template <typename T, typename O> constexpr int kClipBlock = sizeof(O) > sizeof(T) ? 1024 : 256;
+// One tile per block: blocks that come and go keep reads and writes mixed (a grid
+// that loops streams 10-15% slower).  A vector is 16 bytes of the wider type: a
+// lane that stores two halves of 32 bytes leaves every store instruction with gaps
+// (5.4 against 6.5 TB/s).  Blocks of 256 threads with a vector each lead where the
+// types are equal (368M f32: 451 us, with two vectors 476, 512 threads 464, 1024
+// threads 478), with two each where the output is wider, which makes the reads 16
+// bytes too (267M bf16: 252 us, one vector 276, 1024 threads with one 262).
+constexpr int kClipBlock = 256;
 template <typename T, typename O> constexpr int kPair = sizeof(T) > sizeof(O) ? kWidth<T> : kWidth<O>;
+template <typename T, typename O> constexpr int kClipVecs = sizeof(O) > sizeof(T) ? 2 : 1;
+template <typename T, typename O> constexpr unsigned kClipTile = kClipBlock * kPair<T, O> * kClipVecs<T, O>;
 
 // One wave of a block forms c while the block's loads are on their way; the others
 // wait for it rather than do the 64-bit root and quotient as well.
 template <typename T, typename O, bool OWN_OUT>
-__global__ __launch_bounds__((kClipBlock<T, O>)) void k_grad_clip(List<OWN_OUT> l, const double* sumsq, int nsum,
-                                                                  double scale, double max_norm, double* norm) {
-  constexpr int W = kPair<T, O>;
-  constexpr unsigned kTile = kClipBlock<T, O> * W;
+__global__ __launch_bounds__(kClipBlock) void k_grad_clip(List<OWN_OUT> l, const double* sumsq, int nsum,
+                                                          double scale, double max_norm, double* norm) {
+  constexpr int W = kPair<T, O>, U = kClipVecs<T, O>;
   __shared__ double shared_c;
-  const Place<T, O> at = find<kTile, T, O>(l, blockIdx.x);
+  const Place<T, O> at = find<kClipTile<T, O>, T, O>(l, blockIdx.x);
   const T* p = at.p;
   O* o = at.o;
-  const unsigned left = at.left, e = threadIdx.x * W;
-  const bool whole = e + W <= left;
-  Raw<T, W> raw;
-  if (whole) raw.load(p + e);                      // on its way while c is formed
+  Raw<T, W> raw[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const unsigned e = (u * kClipBlock + threadIdx.x) * W;
+    if (e + W <= at.left) raw[u].load(p + e);      // on its way while c is formed
+  }
   if (threadIdx.x < 64) {
     double nrm;
     const double c = coefficient(sumsq, nsum, scale, max_norm, &nrm);
@@ -331,15 +335,19 @@ __global__ __launch_bounds__((kClipBlock<T, O>)) void k_grad_clip(List<OWN_OUT> 
   // in place, a step that is not clipped needs no writes
   if constexpr (std::is_same_v<T, O>)
     if (o == p && c == 1.0) return;
-  if (whole) {
-    T x[W];
-    O y[W];
-    raw.get(x);
 #pragma unroll
-    for (int i = 0; i < W; ++i) y[i] = from_f64<O>(to_f64(x[i]) * c);
-    store(o + e, y);
-  } else {
-    for (unsigned i = e; i < left; ++i) o[i] = from_f64<O>(to_f64(p[i]) * c);
+  for (int u = 0; u < U; ++u) {
+    const unsigned e = (u * kClipBlock + threadIdx.x) * W;
+    if (e + W <= at.left) {
+      T x[W];
+      O y[W];
+      raw[u].get(x);
+#pragma unroll
+      for (int i = 0; i < W; ++i) y[i] = from_f64<O>(to_f64(x[i]) * c);
+      store(o + e, y);
+    } else {
+      for (unsigned i = e; i < at.left; ++i) o[i] = from_f64<O>(to_f64(p[i]) * c);
+    }
   }
 }
 
@@ -633,10 +641,10 @@ int sumsq_t(const void* const* grads, const size_t* ns, int k, double* sumsq, do
 template <typename T, typename O, bool OWN_OUT>
 int clip_lists(void* const* outs, const void* const* grads, const size_t* ns, int k, const double* sumsq, int nsum,
                double scale, double max_norm, double* norm, hipStream_t s) {
-  constexpr unsigned kTile = kClipBlock<T, O> * kPair<T, O>;
+  constexpr unsigned kTile = kClipTile<T, O>;
   bool any = false;
   auto launch = [&](const List<OWN_OUT>& l) {
-    hipLaunchKernelGGL((k_grad_clip<T, O, OWN_OUT>), dim3(tiles_of<kTile>(l)), dim3(kClipBlock<T, O>), 0, s, l, sumsq, nsum,
+    hipLaunchKernelGGL((k_grad_clip<T, O, OWN_OUT>), dim3(tiles_of<kTile>(l)), dim3(kClipBlock), 0, s, l, sumsq, nsum,
                        scale, max_norm, any ? nullptr : norm);
     any = true;
     return launched("grad_clip");
