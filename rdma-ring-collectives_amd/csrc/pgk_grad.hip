@@ -404,13 +404,14 @@ __device__ __forceinline__ O fold_one(const Sources& src, int nsrc, size_t e, do
 // blocks as the workspace holds sums of.  Blocks of 1024 threads lose least by
 // that: 75.6 us for 3 f32 sources of 30M elements (256 threads 83, two launches
 // of 512 threads 79), 95.8 us for 4 f16 sources of 50M to f32 (105, 98); fetching
-// the next vectors ahead makes it slower.  An output whose sum is wanted stays in
-// the caches, as far as it fits, for the clip that follows: 3 f32 sources of 30M
-// elements take 85 instead of 79 us, with the clip 114 instead of 120.
+// the next vectors ahead makes it slower.  stay: an output whose sum is wanted and
+// that fits the Infinity Cache is left there for the clip that follows: 3 f32
+// sources of 30M elements take 85 instead of 79 us, with the clip 114 instead of
+// 120 (an output of 600 MB would only lose, 344 against 304).
 constexpr int kFoldBlock = 1024;
 template <typename T, typename O, int NS>
 __global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, int nsrc, size_t e0, size_t e1,
-                                                          double scale, double* parts, int held) {
+                                                          double scale, double* parts, int held, int stay) {
   constexpr int W = kPair<T, O>;
   double sq = 0.0;
   for (size_t e = e0 + ((size_t)blockIdx.x * kFoldBlock + threadIdx.x) * W; e < e1;
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, i
     if (e + W <= e1) {
       O y[W];
       fold<T, O, NS>(y, src, nsrc, e, scale, &sq);
-      if (parts) store<false>(out + e, y);
+      if (stay) store<false>(out + e, y);
       else store(out + e, y);
     } else {
       for (size_t i = e; i < e1; ++i) out[i] = fold_one<T, O>(src, nsrc, i, scale, &sq);
@@ -710,10 +711,11 @@ int fold_t(void* out, const Sources& src, int nsrc, size_t n, double scale, doub
     constexpr size_t per = (size_t)kFoldBlock * kPair<T, O>;
     const size_t tiles = (n - e0 + per - 1) / per;
     const unsigned grid = one ? 1 : tiles < (size_t)kMaxParts ? (unsigned)tiles : kMaxParts;
+    const int stay = parts && n * sizeof(O) <= kInfinityCache;
     switch (nsrc) {
 #define PGK_FOLD_CASE(NS, K) \
       K: hipLaunchKernelGGL((k_grad_fold<T, O, NS>), dim3(grid), dim3(kFoldBlock), 0, s, o, src, nsrc, e0, n, scale, \
-                            parts, held); break;
+                            parts, held, stay); break;
       PGK_FOLD_CASE(1, case 1) PGK_FOLD_CASE(2, case 2) PGK_FOLD_CASE(3, case 3) PGK_FOLD_CASE(4, case 4)
       PGK_FOLD_CASE(5, case 5) PGK_FOLD_CASE(6, case 6) PGK_FOLD_CASE(7, case 7) PGK_FOLD_CASE(kMaxUnrolled, default)
 #undef PGK_FOLD_CASE
