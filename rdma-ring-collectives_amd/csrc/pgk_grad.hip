@@ -116,8 +116,8 @@ __device__ __forceinline__ O from_f64(double x) {
 // large one 4 to 7, so as many tensors as 4 KiB of kernel arguments can say go
 // into one: an address is 48 bits, and one word holds both a tensor's first tile
 // and how many elements its last tile has.  A tile is what a block takes at a
-// time; every tensor starts one.  A launch ends at 2^(32 - kBits) tiles (8 GiB),
-// a tensor that is longer goes on in the next.
+// time; every tensor starts one.  A launch takes at most 2^32 elements, a longer
+// tensor goes on in the next.
 constexpr int kBuckets = 128;
 
 // Outputs that lie as the gradients do (in place, or two flat buffers with equal
@@ -495,7 +495,7 @@ bool check_list(const char* what, const void* const* p, const size_t* ns, int k,
     if (!ns[j]) continue;
     if (!p[j]) { set_err("pgk: %s: NULL tensor %d with n=%zu", what, j, ns[j]); return false; }
     if (misaligned(p[j], es)) { set_err("pgk: %s: tensor %d is not on a multiple of its element size", what, j); return false; }
-    if ((uintptr_t)p[j] >> 48) { set_err("pgk: %s: tensor %d at %p", what, j, p[j]); return false; }
+    if ((uintptr_t)p[j] >> 48) { set_err("pgk: %s: tensor %d: %p is no device address", what, j, p[j]); return false; }
     if (ns[j] > ((size_t)1 << 40)) { set_err("pgk: %s: tensor %d of %zu elements", what, j, ns[j]); return false; }
   }
   return true;

@@ -59,6 +59,7 @@ def test_lists(lib):
     refused(lib, lib.pgk_grad_sumsq(g, None, 1, F32, SUM, WORK, None), "list")
     refused(lib, lib.pgk_grad_sumsq(ptrs(BASE, None), sizes(4, 1), 2, F32, SUM, WORK, None), "NULL tensor 1")
     refused(lib, lib.pgk_grad_sumsq(g, sizes((1 << 40) + 1), 1, F32, SUM, WORK, None), "elements")
+    refused(lib, lib.pgk_grad_sumsq(ptrs(1 << 48), n, 1, F32, SUM, WORK, None), "no device address")
     refused(lib, lib.pgk_grad_clip(None, F32, g, F32, n, 1, SUM, 1, 1.0, 1.0, None, None), "list")
     refused(lib, lib.pgk_grad_clip(ptrs(None), F32, g, F32, n, 1, SUM, 1, 1.0, 1.0, None, None), "NULL tensor 0")
     refused(lib, lib.pgk_grad_fold(BASE, F32, None, 2, 4, F32, 1.0, None, None, None), "NULL list")

@@ -177,9 +177,10 @@ def allowed(want, out_dt, nsum):
 @pytest.mark.parametrize("dt,out_dt", PAIRS)
 @pytest.mark.parametrize("which", list(LISTS))
 def test_clip(gpu, lib, which, dt, out_dt):
-    for gap, scale, sums in ((0, 1.0, [4.0]), (3, 1 / 3, [0.3, 1e-9, 700.0]), (1, -2.0, [1e-3])):
+    # outputs that lie to each other as the gradients do, and outputs that do not
+    for gap, out_gap, scale, sums in ((0, 0, 1.0, [4.0]), (3, 3, 1 / 3, [0.3, 1e-9, 700.0]), (1, 2, -2.0, [1e-3])):
         _, ts = bucket(LISTS[which], dt, 23 + gap, gap)
-        out, outs = bucket(LISTS[which], out_dt, 1, gap, pad=7.0)
+        out, outs = bucket(LISTS[which], out_dt, 1, out_gap, pad=7.0)
         norm = clip(lib, outs, out_dt, ts, dt, torch.tensor(sums, dtype=torch.float64, device="cuda"), scale, 1.5)
         want_norm, c = coefficient(sums, scale, 1.5)
         assert abs(float(norm) - want_norm) <= (len(sums) + 2) * U * want_norm
@@ -321,6 +322,54 @@ def test_fold_into_a_source(gpu, lib, dt):
         want = plain_fold(srcs, 0.25, dt)
         fold(lib, srcs[into], dt, srcs, dt, 0.25)
         assert torch.equal(srcs[into].cpu(), want)
+
+
+def large_sources(n, dt, nsrc, off=0):
+    g = torch.Generator(device="cuda").manual_seed(n + nsrc)
+    return [torch.randn(n + off, generator=g, device="cuda").to(TYPES[dt][1])[off:] for _ in range(nsrc)]
+
+
+def large_fold(srcs, scale, out_dt):
+    """plain_fold with torch's f64 operations on the GPU, which round as the host's do."""
+    acc = srcs[0].double()
+    for s in srcs[1:]:
+        acc = acc + s.double()
+    acc = acc * scale
+    return (acc.float() if out_dt in ("f16", "bf16") else acc).to(TYPES[out_dt][1])
+
+
+MIB = 1 << 20
+# bytes per source: the burst form takes 64 MiB at a time, then 32 to 64, the rest one vector per thread
+BURST = [(5, 32 * MIB), (6, 32 * MIB + 16), (7, 64 * MIB), (8, 64 * MIB + 40 * MIB), (8, 100 * MIB + 24), (5, 31 * MIB)]
+
+
+@pytest.mark.parametrize("dt", list(TYPES))
+@pytest.mark.parametrize("nsrc,nbytes", BURST)
+@pytest.mark.parametrize("off", [0, 1])
+def test_fold_of_large_blocks(gpu, lib, dt, nsrc, nbytes, off):
+    n = nbytes // torch.finfo(TYPES[dt][1]).bits * 8 + off
+    srcs = large_sources(n, dt, nsrc, off)
+    want = large_fold(srcs, 1.0 / nsrc, dt)
+    out = torch.full((n + 2,), 7.0, dtype=TYPES[dt][1], device="cuda")
+    s = fold(lib, out[1:n + 1], dt, srcs, dt, 1.0 / nsrc)
+    assert torch.equal(out[1:n + 1], want)
+    assert float(out[0]) == 7.0 and float(out[-1]) == 7.0
+    sq = math.fsum(float((part.double() ** 2).sum()) for part in want.split(1 << 16))
+    assert near_sum(s, sq, n + (1 << 16))                 # torch's partial sums are off by up to 2^16 roundings
+    fold(lib, srcs[nsrc - 2], dt, srcs, dt, 1.0 / nsrc, want_sum=False)      # into a source
+    assert torch.equal(srcs[nsrc - 2], want)
+
+
+@pytest.mark.parametrize("dt,out_dt", PAIRS)
+@pytest.mark.parametrize("nsrc,n", [(2, 40_000_003), (3, 70_000_001), (9, 36_000_007)])
+def test_fold_of_more_tiles_than_blocks(gpu, lib, dt, out_dt, nsrc, n):
+    srcs = large_sources(n, dt, nsrc)
+    out = torch.empty(n, dtype=TYPES[out_dt][1], device="cuda")
+    s = fold(lib, out, out_dt, srcs, dt, 0.3)
+    want = large_fold(srcs, 0.3, out_dt)
+    assert torch.equal(out, want)
+    sq = math.fsum(float((part.double() ** 2).sum()) for part in want.split(1 << 16))
+    assert near_sum(s, sq, n + (1 << 16))
 
 
 def test_fold_of_nothing(gpu, lib):
