@@ -596,12 +596,14 @@ int finish(const char* what, const double* work, int held, double* sumsq, hipStr
 }
 
 // Up to here one block of 1024 threads does a call in one launch, without a second
-// one to join the sums of several blocks: 256 KiB of f32 in 5.9 us against 7.6 (512 KiB:
-// 8.6 against 7.6), 2 sources of 80 KB folded in 6.3 us against 7.2.  Joining them in
+// one to join the sums of several blocks.  A norm of 256 KiB of f32 takes it 5.4 us
+// against 7.0 (512 KiB: 8.6 against 7.6); a fold of 480 KB in all, whose loads wait
+// for each other less, 6.4 against 6.9 (720 KB: 8.5 against 6.9).  Joining the sums in
 // the same launch, by the block that finishes last, loses from 128 blocks on: their
 // counter is one address across eight dies (1024 blocks 37 us, two launches 10.3).
-constexpr size_t kOneBlock = 256u << 10;
+constexpr size_t kOneBlockNorm = 256u << 10;
 constexpr size_t kOneBlockTile = 64u << 10;       // what it takes at a time, 4 vectors per thread
+constexpr size_t kOneBlockFold = 512u << 10;
 constexpr size_t kInfinityCache = 256u << 20;
 
 // The blocks of a norm launch: 3 of 256 threads per CU (4 for f64) lead, and leave
@@ -634,7 +636,7 @@ int sumsq_t(const void* const* grads, const size_t* ns, int k, double* sumsq, do
     tiles += (ns[j] * sizeof(T) + kOneBlockTile - 1) / kOneBlockTile;
     bytes += ns[j] * sizeof(T);
   }
-  if (tiles <= kOneBlock / kOneBlockTile) return sumsq_shape<T, 1024, 4, false>(grads, ns, k, sumsq, work, true, s);
+  if (tiles <= kOneBlockNorm / kOneBlockTile) return sumsq_shape<T, 1024, 4, false>(grads, ns, k, sumsq, work, true, s);
   if (bytes <= kInfinityCache) return sumsq_shape<T, 256, 4, false>(grads, ns, k, sumsq, work, false, s);
   return sumsq_shape<T, 256, 4, true>(grads, ns, k, sumsq, work, false, s);
 }
@@ -679,7 +681,7 @@ template <typename T, typename O>
 int fold_t(void* out, const Sources& src, int nsrc, size_t n, double scale, double* sumsq, double* work,
            hipStream_t s) {
   O* o = (O*)out;
-  const bool one = n * (nsrc * sizeof(T) + sizeof(O)) <= kOneBlock;
+  const bool one = n * (nsrc * sizeof(T) + sizeof(O)) <= kOneBlockFold;
   double* parts = !sumsq ? nullptr : one && n ? sumsq : work;
   size_t e0 = 0;
   int held = 0;
