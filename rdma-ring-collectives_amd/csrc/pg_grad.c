@@ -14,6 +14,16 @@
 #include "pg_impl.h"
 #include "pgk_impl.h"
 
+/* 0 when every tensor is device memory (a kernel that read anything else would fault), -1 with the error set. */
+static int check_device(const void *const *p, const size_t *ns, int k, const char *what) {
+  for (int j = 0; j < k; ++j)
+    if (ns[j] && !pg_is_device_ptr(p[j])) {
+      pg_set_error("pg_grad_clip: %s %d is not device memory", what, j);
+      return -1;
+    }
+  return 0;
+}
+
 /* This rank's sum of squares into *sum; 0, or -1 with the error set. */
 static int local_sum(struct pg_impl *im, const void *const *grads, int dt, const size_t *ns, int k, double *sum) {
   if (pg_wait_producers(im, 0) || pg_ensure(&im->gwork, &im->gwork_cap, PGK_GRAD_WORK_BYTES + sizeof(double)))
@@ -37,7 +47,8 @@ int pg_grad_clip(void *const *outs, int out_dt, const void *const *grads, int dt
   double sums[2] = {0.0, 0.0};                    /* sum of squares, ranks that failed */
   int bad = pgk_grad_clip_check(outs, out_dt, grads, dt, ns, k, scale, max_norm);
   if (bad) pg_set_error("pg_grad_clip: %s", pgk_last_error());
-  else bad = local_sum(im, grads, dt, ns, k, &sums[0]);
+  else bad = check_device(grads, ns, k, "gradient") || check_device((const void *const *)outs, ns, k, "output") ||
+             local_sum(im, grads, dt, ns, k, &sums[0]);
   if (bad) { sums[0] = 0.0; sums[1] = 1.0; }
   if (pg->world_size > 1) {
     char mine[256];

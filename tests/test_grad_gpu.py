@@ -178,7 +178,8 @@ def allowed(want, out_dt, nsum):
 @pytest.mark.parametrize("which", list(LISTS))
 def test_clip(gpu, lib, which, dt, out_dt):
     # outputs that lie to each other as the gradients do, and outputs that do not
-    for gap, out_gap, scale, sums in ((0, 0, 1.0, [4.0]), (3, 3, 1 / 3, [0.3, 1e-9, 700.0]), (1, 2, -2.0, [1e-3])):
+    for gap, out_gap, scale, sums in ((0, 0, 1.0, [4.0]), (3, 3, 1 / 3, [0.3, 1e-9, 700.0]), (1, 2, -2.0, [1e-3]),
+                                      (0, 1, 0.7, [1.0]), (2, 0, 0.7, [9.0])):
         _, ts = bucket(LISTS[which], dt, 23 + gap, gap)
         out, outs = bucket(LISTS[which], out_dt, 1, out_gap, pad=7.0)
         norm = clip(lib, outs, out_dt, ts, dt, torch.tensor(sums, dtype=torch.float64, device="cuda"), scale, 1.5)
@@ -191,6 +192,32 @@ def test_clip(gpu, lib, which, dt, out_dt):
         for o in outs:
             inside[o.storage_offset():o.storage_offset() + o.numel()] = True
         assert (out.cpu()[~inside].double() == 7.0).all()      # what lies between the outputs stays
+
+
+@pytest.mark.parametrize("nsum", [2, 63, 64, 65, 1000])
+def test_clip_by_many_partial_sums(gpu, lib, nsum):
+    sums = [0.001 * (1 + j % 7) for j in range(nsum)]
+    _, ts = bucket([3000, 1], "f32", nsum)
+    outs = [torch.empty_like(t) for t in ts]
+    norm = clip(lib, outs, "f32", ts, "f32", torch.tensor(sums, dtype=torch.float64, device="cuda"), 1.0, 0.01)
+    want_norm, c = coefficient(sums, 1.0, 0.01)
+    assert abs(float(norm) - want_norm) <= (nsum + 2) * U * want_norm
+    for t, o in zip(ts, outs):
+        want = t.cpu().double() * c
+        assert ((o.cpu().double() - want).abs() <= allowed(want, "f32", nsum)).all()
+
+
+def test_clip_bits_do_not_depend_on_the_layout(gpu, lib):
+    """Adjacent tensors are clipped as one; the results are those of the same tensors apart."""
+    numels = [5, 4097, 1, 0, 70_001, 3]
+    _, apart = bucket(numels, "bf16", 12, 3, pad=0.0)
+    flat = torch.cat(apart)
+    together = list(flat.split(numels))
+    s = sumsq(lib, apart, "bf16")
+    assert torch.equal(sumsq(lib, together, "bf16"), s)      # and the norm's bits do not either
+    clip(lib, apart, "bf16", apart, "bf16", s, 0.3, 1.0)
+    clip(lib, together, "bf16", together, "bf16", s, 0.3, 1.0)
+    assert torch.equal(torch.cat(apart), flat)
 
 
 @pytest.mark.parametrize("dt,out_dt", PAIRS)
@@ -322,6 +349,16 @@ def test_fold_into_a_source(gpu, lib, dt):
         want = plain_fold(srcs, 0.25, dt)
         fold(lib, srcs[into], dt, srcs, dt, 0.25)
         assert torch.equal(srcs[into].cpu(), want)
+
+
+@pytest.mark.parametrize("nsrc", [3, 9])
+def test_fold_of_a_source_that_is_listed_twice(gpu, lib, nsrc):
+    x = bucket([10_001], "f32", 4, 1)[1][0]
+    y = bucket([10_001], "f32", 5, 2)[1][0]
+    srcs = [x, y] + [x] * (nsrc - 2)
+    want = plain_fold(srcs, 0.5, "f32")
+    fold(lib, x, "f32", srcs, "f32", 0.5)
+    assert torch.equal(x.cpu(), want)
 
 
 def large_sources(n, dt, nsrc, off=0):
@@ -477,6 +514,30 @@ def test_fold_captured_and_replayed(gpu, lib):
         assert near_sum(s, sq, 70_003)
         torch.ones(1000, device="cuda").sum()
         torch.cuda.synchronize()
+
+
+def test_two_graphs_that_share_a_workspace(gpu, lib):
+    """Replayed one behind the other on one stream, with eager calls on the same workspace between them."""
+    ws, side = work(), torch.cuda.Stream()
+    sets = [bucket([200_003, 9], "f32", 100 + k)[1] for k in range(2)]
+    cells, lists, graphs = [cell() for _ in sets], [(ptrs(ts), sizes(ts)) for ts in sets], []
+    torch.cuda.synchronize()
+    for k in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+            assert lib.pgk_grad_sumsq(*lists[k], 2, pgamd.DT_F32, cells[k].data_ptr(), ws.data_ptr(), stream()) == 0
+        graphs.append(g)
+    want = [exact_sumsq(ts) for ts in sets]
+    for rep in range(3):
+        for c in cells:
+            c.fill_(math.nan)
+        graphs[0].replay()
+        graphs[1].replay()
+        eager = sumsq(lib, sets[1], "f32", ws=ws)
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        assert near_sum(cells[0], want[0], 200_012) and near_sum(cells[1], want[1], 200_012)
+        assert torch.equal(eager, cells[1])
 
 
 def test_two_streams_with_a_workspace_each(gpu, lib):

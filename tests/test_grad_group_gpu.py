@@ -98,6 +98,21 @@ def test_one_rank(gpu, lib):
         lib.pg_close(h)
 
 
+def test_host_memory_is_refused(gpu, lib):
+    h = ctypes.c_void_p()
+    pgamd.check(lib.pg_connect_local(0, 1, pgamd.PG_TRANSPORT_SELF, ctypes.byref(h)), "pg_connect_local")
+    try:
+        dev, host = gpu.ones(8, device="cuda"), gpu.ones(8)
+        d, ns, _ = pgamd.tensor_list([dev])
+        o = pgamd.tensor_list([host])[0]
+        for out, grad, word in ((d, o, "gradient 0"), (o, d, "output 0")):
+            assert lib.pg_grad_clip(out, pgamd.DT_F32, grad, pgamd.DT_F32, ns, 1, 1.0, 1.0, None, h) == -1
+            assert f"{word} is not device memory" in pgamd.last_error()
+        assert bool((dev == 1).all()) and bool((host == 1).all())
+    finally:
+        lib.pg_close(h)
+
+
 def test_gradients_produced_on_the_null_stream(gpu, lib):
     """Work on torch's default stream that is still running when the call is entered is waited for."""
     torch = gpu
