@@ -15,12 +15,14 @@
 #include "pgk_impl.h"
 
 /* 0 when every tensor is device memory (a kernel that read anything else would fault), -1 with the error set. */
-static int check_device(const void *const *p, const size_t *ns, int k, const char *what) {
-  for (int j = 0; j < k; ++j)
-    if (ns[j] && !pg_is_device_ptr(p[j])) {
-      pg_set_error("pg_grad_clip: %s %d is not device memory", what, j);
-      return -1;
-    }
+static int check_device(void *const *outs, const void *const *grads, const size_t *ns, int k) {
+  for (int j = 0; j < k; ++j) {
+    if (!ns[j]) continue;
+    const int grad = pg_is_device_ptr(grads[j]);
+    if (grad && (outs[j] == grads[j] || pg_is_device_ptr(outs[j]))) continue;
+    pg_set_error("pg_grad_clip: %s %d is not device memory", grad ? "output" : "gradient", j);
+    return -1;
+  }
   return 0;
 }
 
@@ -47,8 +49,7 @@ int pg_grad_clip(void *const *outs, int out_dt, const void *const *grads, int dt
   double sums[2] = {0.0, 0.0};                    /* sum of squares, ranks that failed */
   int bad = pgk_grad_clip_check(outs, out_dt, grads, dt, ns, k, scale, max_norm);
   if (bad) pg_set_error("pg_grad_clip: %s", pgk_last_error());
-  else bad = check_device(grads, ns, k, "gradient") || check_device((const void *const *)outs, ns, k, "output") ||
-             local_sum(im, grads, dt, ns, k, &sums[0]);
+  else bad = check_device(outs, grads, ns, k) || local_sum(im, grads, dt, ns, k, &sums[0]);
   if (bad) { sums[0] = 0.0; sums[1] = 1.0; }
   if (pg->world_size > 1) {
     char mine[256];
@@ -63,8 +64,8 @@ int pg_grad_clip(void *const *outs, int out_dt, const void *const *grads, int dt
     return -1;
   }
 
-  double *dsum = (double *)((char *)im->gwork + PGK_GRAD_WORK_BYTES);
-  PG_CHECK_HIP(hipMemcpyAsync(dsum, sums, sizeof(double), hipMemcpyHostToDevice, im->red));
+  double *dsum = (double *)((char *)im->gwork + PGK_GRAD_WORK_BYTES);       /* holds this rank's sum */
+  if (pg->world_size > 1) PG_CHECK_HIP(hipMemcpyAsync(dsum, sums, sizeof(double), hipMemcpyHostToDevice, im->red));
   int rc = pgk_grad_clip(outs, out_dt, grads, dt, ns, k, dsum, 1, scale, max_norm, NULL, (void *)im->red);
   if (rc) pg_set_error("pg_grad_clip: %s", pgk_last_error());
   if (pg_stream_wait(im->red) || rc) return -1;
