@@ -184,16 +184,12 @@ def _plain_fold(srcs, out):
 
 # ---- one pass --------------------------------------------------------------------------------------
 
-_loaded = []
-
-
 def _library():
-    """The binding and the library, loaded by the first call as a program's import does."""
-    if not _loaded:
-        sys.path.insert(0, str(pathlib.Path(__file__).resolve().parents[1] / "rdma-ring-collectives_amd"))
-        import pgamd
-        _loaded.extend((pgamd, pgamd.load()))
-    return _loaded
+    at = str(pathlib.Path(__file__).resolve().parents[1] / "rdma-ring-collectives_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    import pgamd
+    return pgamd, pgamd.load()
 
 
 def _own_sumsq(state):
