@@ -30,6 +30,7 @@ PG_COLL_REDUCE_SCATTER, PG_COLL_ALL_GATHER, PG_COLL_ALL_REDUCE = 0, 1, 2
 PGK_STAGED_MAX_BYTES = 16 << 20
 DT_F32, DT_F16, DT_BF16 = 2, 3, 4                  # gradient types of pgk_grad_* beside DT_DOUBLE
 PGK_GRAD_WORK_BYTES = 65536
+_TORCH_NAMES = {DT_DOUBLE: "torch.float64", DT_F32: "torch.float32", DT_F16: "torch.float16", DT_BF16: "torch.bfloat16"}
 
 ELEM_SIZE = {DT_INT32: 4, DT_DOUBLE: 8}
 
@@ -250,12 +251,27 @@ def plan_coalesce(steps, es):
     return [{name: getattr(out[i], name) for name, _ in PgRedRange._fields_} for i in range(k)]
 
 
-def tensor_list(tensors):
+def tensor_list(tensors, dt=None):
     """(pointers, element counts, number) of contiguous torch tensors, as the
-    pgk_grad_* calls take them.  It holds no reference: keep the tensors."""
+    pgk_grad_* calls take them.  It holds no reference: keep the tensors.
+
+    The calls believe the type code that comes with a list, and a kernel reads
+    whatever addresses are in it.  With `dt` (DT_DOUBLE, DT_F32, DT_F16 or
+    DT_BF16), the code that the call will get, every tensor has to be GPU memory
+    of that type.  Without it a list that has GPU tensors in it has one type and
+    one device."""
+    if dt is not None and dt not in _TORCH_NAMES:
+        raise ValueError(f"type {dt} is no gradient type")
+    first = next((t for t in tensors if t.is_cuda), None)
     for i, t in enumerate(tensors):
         if not t.is_contiguous():
             raise ValueError(f"tensor {i} is not contiguous")
+        if dt is not None and str(t.dtype) != _TORCH_NAMES[dt]:
+            raise ValueError(f"tensor {i} is {t.dtype}, not {_TORCH_NAMES[dt]}")
+        if dt is not None and not t.is_cuda:
+            raise ValueError(f"tensor {i} is on {t.device}, not GPU memory")
+        if first is not None and (t.dtype, t.device) != (first.dtype, first.device):
+            raise ValueError(f"tensor {i} is {t.dtype} on {t.device}, others are {first.dtype} on {first.device}")
     k = len(tensors)
     pointers = (ctypes.c_void_p * max(k, 1))(*[t.data_ptr() or None for t in tensors])
     return pointers, (ctypes.c_size_t * max(k, 1))(*[t.numel() for t in tensors]), k
