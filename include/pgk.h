@@ -166,6 +166,8 @@ PG_API int pgk_all_reduce_staged(void *const *sendbufs, void *const *recvbufs, i
  * call uses it until it has run on its stream; calls that may overlap in time
  * (two streams, two graphs replayed at once) need one each.
  *
+ * work, sumsq and norm lie outside the call's tensors (refused otherwise).
+ *
  * Results depend on the values, the sizes and the order of the tensors and the
  * GPU's number of CUs only: the same call gives the same bits. */
 #define PGK_DT_F32  2

@@ -512,6 +512,15 @@ bool check_work(const char* what, const double* sumsq, const void* work) {
   return true;
 }
 
+// Whether a result's or the workspace's place lies in none of the tensors: kernels that
+// read or write them are on their way while it is written.
+bool check_apart(const char* what, const char* name, const void* p, size_t bytes, const void* const* ts,
+                 const size_t* ns, int k, size_t es) {
+  for (int j = 0; j < k; ++j)
+    if (ns[j] && overlap(p, bytes, ts[j], ns[j] * es)) { set_err("pgk: %s: %s lies in tensor %d", what, name, j); return false; }
+  return true;
+}
+
 int launched(const char* what) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) { set_err("pgk: %s: launch failed: %s", what, hipGetErrorString(e)); return -1; }
@@ -759,7 +768,8 @@ int pgk_grad_sumsq(const void* const* grads, const size_t* ns, int k, int dt, do
                    void* stream) {
   const char* what = "grad_sumsq";
   if (!check_types(what, dt, dt) || !check_list(what, grads, ns, k, elem_size(dt)) ||
-      !check_work(what, sumsq, work)) return -1;
+      !check_work(what, sumsq, work) || !check_apart(what, "sumsq", sumsq, 8, grads, ns, k, elem_size(dt)) ||
+      !check_apart(what, "work", work, PGK_GRAD_WORK_BYTES, grads, ns, k, elem_size(dt))) return -1;
   return with_types(dt, dt, [&](auto* t, auto*) {
     return sumsq_t<std::remove_pointer_t<decltype(t)>>(grads, ns, k, sumsq, (double*)work, (hipStream_t)stream);
   });
@@ -788,6 +798,10 @@ int pgk_grad_clip(void* const* outs, int out_dt, const void* const* grads, int d
       (norm && !check_sums(what, norm, "norm"))) return -1;
   if (nsum < 1) { set_err("pgk: %s: %d partial sums", what, nsum); return -1; }
   if (norm && overlap(norm, 8, sumsq, (size_t)nsum * 8)) { set_err("pgk: %s: norm lies in sumsq", what); return -1; }
+  const void* const* const o = (const void* const*)outs;
+  if (!check_apart(what, "sumsq", sumsq, (size_t)nsum * 8, o, ns, k, elem_size(out_dt)) ||
+      (norm && (!check_apart(what, "norm", norm, 8, o, ns, k, elem_size(out_dt)) ||
+                !check_apart(what, "norm", norm, 8, grads, ns, k, elem_size(dt))))) return -1;
   return with_types(dt, out_dt, [&](auto* t, auto* o) {
     return clip_t<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(o)>>(
         outs, grads, ns, k, sumsq, nsum, scale, max_norm, norm, (hipStream_t)stream);
@@ -816,6 +830,10 @@ int pgk_grad_fold(void* out, int out_dt, const void* const* srcs, int nsrc, size
         return -1;
       }
     }
+    if (sumsq && (!check_apart(what, "sumsq", sumsq, 8, o, same, 1, oes) ||
+                  !check_apart(what, "sumsq", sumsq, 8, srcs, same, nsrc, es) ||
+                  !check_apart(what, "work", work, PGK_GRAD_WORK_BYTES, o, same, 1, oes) ||
+                  !check_apart(what, "work", work, PGK_GRAD_WORK_BYTES, srcs, same, nsrc, es))) return -1;
   } else if (!sumsq) {
     return 0;
   }

@@ -1,6 +1,7 @@
 """Lists and places that the gradient entry points (include/pgk.h, pgk_grad_*) must
 not take, because a kernel would read or write where it should not.  Everything is
 refused on the host, so no GPU is needed."""
+import ctypes
 import types
 
 import pytest
@@ -52,3 +53,62 @@ def test_mixed_lists_on_the_gpu(other):
 def test_types_that_no_gradient_has(dt):
     with pytest.raises(ValueError, match="no gradient type"):
         pgamd.tensor_list([], dt)
+
+
+# ---- places of results and workspace inside the tensors ----------------------------------------------
+
+A, B, C = 0x10_0000_0000, 0x20_0000_0000, 0x30_0000_0000        # addresses far apart; nothing is there to touch
+WORK = pgamd.PGK_GRAD_WORK_BYTES
+PAIRS = [(F64, F64), (F32, F32), (F16, F16), (BF16, BF16), (F16, F32), (BF16, F32)]
+SIZE = {F64: 8, F32: 4, F16: 2, BF16: 2}
+
+
+def ptrs(*p):
+    return (ctypes.c_void_p * len(p))(*p)
+
+
+def sizes(*n):
+    return (ctypes.c_size_t * len(n))(*n)
+
+
+def refused(lib, rc, word):
+    assert rc == -1
+    msg = (lib.pgk_last_error() or b"").decode()
+    assert word in msg, msg
+
+
+@pytest.mark.parametrize("dt", [F64, F32, F16, BF16])
+def test_norm_into_its_gradients(lib, dt):
+    """The last 8 bytes of a tensor, and a workspace that reaches into it from either side."""
+    n = 1000 if dt == F64 else 4000
+    end = B + n * SIZE[dt]
+    g, ns = ptrs(A, 0, B), sizes(16, 0, n)
+    for s in (B, end - 8):
+        refused(lib, lib.pgk_grad_sumsq(g, ns, 3, dt, s, C, None), "sumsq lies in tensor 2")
+    for w in (B - WORK + 8, end - 8):
+        refused(lib, lib.pgk_grad_sumsq(g, ns, 3, dt, C, w, None), "work lies in tensor 2")
+
+
+@pytest.mark.parametrize("dt,out_dt", PAIRS)
+def test_clip_into_its_own_sums(lib, dt, out_dt):
+    n = 4000
+    g, o, ns = ptrs(A, B), ptrs(A + (1 << 20), C), sizes(16, n)
+    end = C + n * SIZE[out_dt]
+    for s, nsum in ((C, 1), (end - 8, 1), (C - 24, 4), (end - 8, 9)):
+        refused(lib, lib.pgk_grad_clip(o, out_dt, g, dt, ns, 2, s, nsum, 1.0, 1.0, None, None), "sumsq lies in tensor 1")
+    s = A + (1 << 21)
+    for norm in (C, end - 8, B, B + n * SIZE[dt] - 8):
+        refused(lib, lib.pgk_grad_clip(o, out_dt, g, dt, ns, 2, s, 1, 1.0, 1.0, norm, None), "norm lies in tensor 1")
+    if dt == out_dt:                                              # in place
+        refused(lib, lib.pgk_grad_clip(g, dt, g, dt, ns, 2, B + 8, 1, 1.0, 1.0, None, None), "sumsq lies in tensor 1")
+
+
+@pytest.mark.parametrize("dt,out_dt", PAIRS)
+def test_fold_into_its_own_sum(lib, dt, out_dt):
+    n = 4000
+    src, s0 = ptrs(A, B), C + (1 << 20)
+    for s in (C, C + n * SIZE[out_dt] - 8):
+        refused(lib, lib.pgk_grad_fold(C, out_dt, src, 2, n, dt, 1.0, s, s0, None), "sumsq lies in tensor 0")
+    refused(lib, lib.pgk_grad_fold(C, out_dt, src, 2, n, dt, 1.0, B + n * SIZE[dt] - 8, s0, None), "sumsq lies in tensor 1")
+    refused(lib, lib.pgk_grad_fold(C, out_dt, src, 2, n, dt, 1.0, s0, C + n * SIZE[out_dt] - 8, None), "work lies in tensor 0")
+    refused(lib, lib.pgk_grad_fold(C, out_dt, src, 2, n, dt, 1.0, s0, B - WORK + 8, None), "work lies in tensor 1")
