@@ -183,8 +183,9 @@ PG_API int pgx_reduce_host(void *dst, const void *src, size_t n, int datatype, i
  * by their global norm: pgk_grad_sumsq over this rank's k tensors, the ranks'
  * sums added up (one pg_all_reduce of two doubles), pgk_grad_clip by the result.
  * include/pgk.h has the types, the formula and what tensors have to be like; here
- * they are device memory of the handle's device, complete or produced on the null
- * stream (as the device buffers of every pg_* call).  Each rank has its own
+ * they are memory of the handle's device, which is the current one (refused
+ * otherwise), complete or produced on the null stream (as the device buffers of
+ * every pg_* call).  Each rank has its own
  * tensors (its reduce-scatter shard, its pipeline stage; none at all with k = 0):
  * a tensor that several ranks hold counts on each of them.  scale and max_norm
  * are the same on every rank.  *norm (host, may be NULL): the norm, the same on

@@ -10,17 +10,36 @@
  */
 #include <math.h>
 #include <stdio.h>
+#include <string.h>
 
 #include "pg_impl.h"
 #include "pgk_impl.h"
 
-/* 0 when every tensor is device memory (a kernel that read anything else would fault), -1 with the error set. */
-static int check_device(void *const *outs, const void *const *grads, const size_t *ns, int k) {
+/* Memory that a kernel on `device` can read and write: that device's, or managed. */
+static int on_device(const void *p, int device) {
+  hipPointerAttribute_t a;
+  memset(&a, 0, sizeof(a));
+  if (hipPointerGetAttributes(&a, p) != hipSuccess) {
+    (void)hipGetLastError();
+    return 0;
+  }
+  return (a.type == hipMemoryTypeDevice && a.device == device) || a.type == hipMemoryTypeManaged || a.isManaged;
+}
+
+/* 0 when the handle's device is the current one, which the workspace is allocated on, and every tensor is
+ * its memory (a kernel that read anything else would fault); -1 with the error set. */
+static int check_device(int device, void *const *outs, const void *const *grads, const size_t *ns, int k) {
+  int current = -1;
+  PG_CHECK_HIP(hipGetDevice(&current));
+  if (current != device) {
+    pg_set_error("pg_grad_clip: the current device is %d, the handle's %d", current, device);
+    return -1;
+  }
   for (int j = 0; j < k; ++j) {
     if (!ns[j]) continue;
-    const int grad = pg_is_device_ptr(grads[j]);
-    if (grad && (outs[j] == grads[j] || pg_is_device_ptr(outs[j]))) continue;
-    pg_set_error("pg_grad_clip: %s %d is not device memory", grad ? "output" : "gradient", j);
+    const int grad = on_device(grads[j], device);
+    if (grad && (outs[j] == grads[j] || on_device(outs[j], device))) continue;
+    pg_set_error("pg_grad_clip: %s %d is not device memory of device %d", grad ? "output" : "gradient", j, device);
     return -1;
   }
   return 0;
@@ -49,7 +68,7 @@ int pg_grad_clip(void *const *outs, int out_dt, const void *const *grads, int dt
   double sums[2] = {0.0, 0.0};                    /* sum of squares, ranks that failed */
   int bad = pgk_grad_clip_check(outs, out_dt, grads, dt, ns, k, scale, max_norm);
   if (bad) pg_set_error("pg_grad_clip: %s", pgk_last_error());
-  else bad = check_device(outs, grads, ns, k) || local_sum(im, grads, dt, ns, k, &sums[0]);
+  else bad = check_device(pg->device, outs, grads, ns, k) || local_sum(im, grads, dt, ns, k, &sums[0]);
   if (bad) { sums[0] = 0.0; sums[1] = 1.0; }
   if (pg->world_size > 1) {
     char mine[256];
