@@ -209,3 +209,40 @@ def test_fold_of_another_process_s_memory(gpu, lib):
         if p.is_alive():
             p.kill()
     assert p.exitcode == 0
+
+
+def _replayed_us(call):
+    """Time of one of 60 calls captured one behind the other, the shortest of nine replays."""
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        for _ in range(60):
+            call()
+    took = []
+    for _ in range(12):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        took.append(a.elapsed_time(b) * 1e3 / 60)
+    return min(took[3:])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("want_sum", [False])
+def test_a_small_fold_takes_no_longer_than_one_of_twice_its_size(gpu, lib, dt, want_sum):
+    """The form of one block is for calls that it makes shorter.  Two sources, 480 KiB in all against 960: where one
+    block took the smaller one, it was 2 to 4 times as long."""
+    took = []
+    for n in (480 * 1024, 960 * 1024):
+        n //= 3 * torch.finfo(TYPES[dt][1]).bits // 8
+        srcs, ws, s = [whole_numbers(n, dt, k) for k in range(2)], work(), cell()
+        out, lst, code = torch.empty_like(srcs[0]), ptrs(srcs), TYPES[dt][0]
+
+        def call():
+            assert lib.pgk_grad_fold(out.data_ptr(), code, lst, 2, n, code, 0.5, s.data_ptr() if want_sum else None,
+                                     ws.data_ptr() if want_sum else None, stream()) == 0
+
+        took.append(_replayed_us(call))
+    assert took[0] <= 1.6 * took[1], took
