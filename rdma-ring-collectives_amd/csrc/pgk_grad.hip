@@ -616,16 +616,19 @@ int finish(const char* what, const double* work, int held, double* sumsq, hipStr
 }
 
 // Up to here one block of 1024 threads does a call in one launch, without a second
-// one to join the sums of several blocks.  A norm of 256 KiB of f32 takes it 5.4 us
-// against 7.0 (512 KiB: 8.6 against 7.6); a fold of 480 KB in all, whose loads wait
-// for each other less, 6.4 against 6.9 (720 KB: 8.5 against 6.9).  A fold without a sum
+// one to join the sums of several blocks.  Called one behind the other, one block or
+// two launches take
+//   a norm of 256 KiB             f32 5.0, 6.2 us   bf16 6.4, 6.2 us
+//   a fold of 2 sources, 256 KiB      4.5, 6.0           6.9, 6.0  (4 sources 6.0, 6.0)
+//   the same, 480 KiB in all          6.2, 6.1          11.0, 6.1
+// as a 16-bit value takes two conversions and half the bytes.  A fold without a sum
 // has none to join: 2 bf16 sources, 480 KiB in all, take many blocks 2.3 us in a graph,
 // one block 10.2.  Joining the sums in the same launch, by the block that finishes last,
 // loses from 128 blocks on: their counter is one address across eight dies (1024 blocks
 // 37 us, two launches 10.3).
 constexpr size_t kOneBlockNorm = 256u << 10;
 constexpr size_t kOneBlockTile = 64u << 10;       // what it takes at a time, 4 vectors per thread
-constexpr size_t kOneBlockFold = 512u << 10;
+template <typename T> constexpr size_t kOneBlockFold = (sizeof(T) == 2 ? 256u : 512u) << 10;
 constexpr size_t kInfinityCache = 256u << 20;
 
 // The blocks of a norm launch: 3 of 256 threads per CU (4 for f64) lead, and leave
@@ -703,7 +706,7 @@ template <typename T, typename O>
 int fold_t(void* out, const Sources& src, int nsrc, size_t n, double scale, double* sumsq, double* work,
            hipStream_t s) {
   O* o = (O*)out;
-  const bool one = sumsq && n * (nsrc * sizeof(T) + sizeof(O)) <= kOneBlockFold;
+  const bool one = sumsq && n * (nsrc * sizeof(T) + sizeof(O)) <= kOneBlockFold<T>;
   double* parts = !sumsq ? nullptr : one && n ? sumsq : work;
   size_t e0 = 0;
   int held = 0;

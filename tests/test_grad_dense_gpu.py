@@ -230,7 +230,7 @@ def _replayed_us(call):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
-@pytest.mark.parametrize("want_sum", [False])
+@pytest.mark.parametrize("want_sum", [False, True])
 def test_a_small_fold_takes_no_longer_than_one_of_twice_its_size(gpu, lib, dt, want_sum):
     """The form of one block is for calls that it makes shorter.  Two sources, 480 KiB in all against 960: where one
     block took the smaller one, it was 2 to 4 times as long."""
