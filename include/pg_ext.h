@@ -189,9 +189,11 @@ PG_API int pgx_reduce_host(void *dst, const void *src, size_t n, int datatype, i
  * tensors (its reduce-scatter shard, its pipeline stage; none at all with k = 0):
  * a tensor that several ranks hold counts on each of them.  scale and max_norm
  * are the same on every rank.  *norm (host, may be NULL): the norm, the same on
- * every rank.  Synchronous.  A rank whose arguments are refused makes the call
- * return -1 on every rank, with every tensor as it was.  world_size == 1 needs no
- * exchange; PG_TRANSPORT_LOOPBACK has no all-reduce and returns -1.
+ * every rank.  Synchronous.  A rank whose arguments are refused, or whose sum
+ * fails, makes the call return -1 on every rank, with every tensor as it was.  A
+ * GPU error behind the exchange of the sums returns -1 on that rank alone; the
+ * others have clipped by then.  world_size == 1 needs no exchange;
+ * PG_TRANSPORT_LOOPBACK has no all-reduce and returns -1.
  * pg_get_stats describes the all-reduce inside. */
 PG_API int pg_grad_clip(void *const *outs, int out_dt, const void *const *grads, int dt, const size_t *ns, int k,
                         double scale, double max_norm, double *norm, void *pg_handle);

@@ -166,7 +166,8 @@ PG_API int pgk_all_reduce_staged(void *const *sendbufs, void *const *recvbufs, i
  * call uses it until it has run on its stream; calls that may overlap in time
  * (two streams, two graphs replayed at once) need one each.
  *
- * work, sumsq and norm lie outside the call's tensors (refused otherwise).
+ * work, sumsq and norm lie outside the call's tensors: what the call would write
+ * while it reads it is refused.
  *
  * Results depend on the values, the sizes and the order of the tensors and the
  * GPU's number of CUs only: the same call gives the same bits. */
@@ -209,8 +210,9 @@ PG_API int pgk_grad_clip(void *const *outs, int out_dt, const void *const *grads
  * sumsq (device, outside work, may be NULL): the sum of the squares of out as
  * stored, what pgk_grad_sumsq over out would give up to the order of its sum,
  * without reading it again; 0 when n = 0.  Without sumsq, work may be NULL.
- * Sources may be peer GPUs' memory as in pgk_reduce_multi; out may be one of them
- * when the types are equal. */
+ * Sources may be peers' memory mapped through HIP IPC, as in pgk_reduce_multi; the
+ * launches are those measured best on local HBM (there is no flag as
+ * PGK_FOLD_REMOTE_SOURCES).  out may be one of the sources when the types are equal. */
 PG_API int pgk_grad_fold(void *out, int out_dt, const void *const *srcs, int nsrc, size_t n, int dt, double scale,
                          double *sumsq, void *work, void *stream);
 

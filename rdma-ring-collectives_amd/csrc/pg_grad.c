@@ -5,8 +5,9 @@
  * The local sum of squares and the clip are kernels (pgk_grad_*); between them
  * the ranks' sums meet in one pg_all_reduce of two doubles, the second of which
  * says how many ranks cannot go on.  A rank whose arguments are refused or
- * whose launch fails takes part in it all the same, so the call fails on every
- * rank and nobody waits for a rank that has left.
+ * whose own sum fails takes part in it all the same, so the call fails on every
+ * rank and nobody waits for a rank that has left.  What fails behind the
+ * all-reduce (the upload of the sum, the clip) fails on that rank alone.
  */
 #include <math.h>
 #include <stdio.h>

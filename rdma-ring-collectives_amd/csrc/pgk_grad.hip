@@ -299,19 +299,18 @@ __device__ __forceinline__ double coefficient(const double* sumsq, int nsum, dou
 // lane that stores two halves of 32 bytes leaves every store instruction with gaps
 // (5.4 against 6.5 TB/s).  Blocks of 256 threads with a vector each lead where the
 // types are equal (368M f32: 451 us, with two vectors 476, 512 threads 464, 1024
-// threads 478), with two each where the output is wider, which makes the reads 16
-// bytes too (267M bf16: 252 us, one vector 276, 1024 threads with one 262).
+// threads 478), with two each where the output is wider, whose reads are of 8 bytes
+// (267M bf16: 252 us, one vector 276, 1024 threads with one 262).
 constexpr int kClipBlock = 256;
-template <typename T, typename O> constexpr int kPair = sizeof(T) > sizeof(O) ? kWidth<T> : kWidth<O>;
 template <typename T, typename O> constexpr int kClipVecs = sizeof(O) > sizeof(T) ? 2 : 1;
-template <typename T, typename O> constexpr unsigned kClipTile = kClipBlock * kPair<T, O> * kClipVecs<T, O>;
+template <typename T, typename O> constexpr unsigned kClipTile = kClipBlock * kWidth<O> * kClipVecs<T, O>;
 
 // One wave of a block forms c while the block's loads are on their way; the others
 // wait for it rather than do the 64-bit root and quotient as well.
 template <typename T, typename O, bool OWN_OUT>
 __global__ __launch_bounds__(kClipBlock) void k_grad_clip(List<OWN_OUT> l, const double* sumsq, int nsum,
                                                           double scale, double max_norm, double* norm) {
-  constexpr int W = kPair<T, O>, U = kClipVecs<T, O>;
+  constexpr int W = kWidth<O>, U = kClipVecs<T, O>;
   __shared__ double shared_c;
   const Place<T, O> at = find<kClipTile<T, O>, T, O>(l, blockIdx.x);
   const T* p = at.p;
@@ -412,7 +411,7 @@ constexpr int kFoldBlock = 1024;
 template <typename T, typename O, int NS>
 __global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, int nsrc, size_t e0, size_t e1,
                                                           double scale, double* parts, int held, int stay) {
-  constexpr int W = kPair<T, O>;
+  constexpr int W = kWidth<O>;
   double sq = 0.0;
   for (size_t e = e0 + ((size_t)blockIdx.x * kFoldBlock + threadIdx.x) * W; e < e1;
        e += (size_t)gridDim.x * kFoldBlock * W) {
@@ -716,7 +715,7 @@ int fold_t(void* out, const Sources& src, int nsrc, size_t n, double scale, doub
     return launched("grad_fold");
   };
   // the launches of the burst form hold what the waves' registers hold: 512 blocks (two per CU) of 32
-  // vectors per thread, then one of 512 to 1023 blocks of 16; what is left, under 32 MiB per source,
+  // vectors per thread, then one of 512 to 1024 blocks of 16; what is left, under 32 MiB per source,
   // goes a vector per thread
   if constexpr (std::is_same_v<T, O>) {
     constexpr size_t kHalf = (size_t)512 * kBurstBlock * 16 * kWidth<T>;      // 32 MiB per source
@@ -735,7 +734,7 @@ int fold_t(void* out, const Sources& src, int nsrc, size_t n, double scale, doub
     }
   }
   if (e0 < n) {
-    constexpr size_t per = (size_t)kFoldBlock * kPair<T, O>;
+    constexpr size_t per = (size_t)kFoldBlock * kWidth<O>;
     const size_t tiles = (n - e0 + per - 1) / per;
     const unsigned grid = one ? 1 : tiles < (size_t)kMaxParts ? (unsigned)tiles : kMaxParts;
     const int stay = parts && n * sizeof(O) <= kInfinityCache;
