@@ -401,16 +401,15 @@ __device__ __forceinline__ O fold_one(const Sources& src, int nsrc, size_t e, do
 
 // Elements [e0, e1), a vector per thread at a time, in a grid of at most as many
 // blocks as the workspace holds sums of.  Blocks of 1024 threads lose least by
-// that: 75.6 us for 3 f32 sources of 30M elements (256 threads 83, two launches
-// of 512 threads 79), 95.8 us for 4 f16 sources of 50M to f32 (105, 98); fetching
-// the next vectors ahead makes it slower.  stay: an output whose sum is wanted and
-// that fits the Infinity Cache is left there for the clip that follows: 3 f32
-// sources of 30M elements take 85 instead of 79 us, with the clip 114 instead of
-// 120 (an output of 600 MB would only lose, 344 against 304).
+// that: 85 us for 3 f32 sources of 30M elements (256 threads 92), 107 us for 4 f16
+// sources of 50M to f32 (118); fetching the next vectors ahead makes it slower.
+// The output is stored with the default policy, for what reads it next: the 30M
+// elements take 85 us, with a clip behind 114; past the caches 79 and 120.  An output
+// of 600 MiB takes 344 and 507, past the caches 324 and 518.
 constexpr int kFoldBlock = 1024;
 template <typename T, typename O, int NS>
 __global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, int nsrc, size_t e0, size_t e1,
-                                                          double scale, double* parts, int held, int stay) {
+                                                          double scale, double* parts, int held) {
   constexpr int W = kWidth<O>;
   double sq = 0.0;
   for (size_t e = e0 + ((size_t)blockIdx.x * kFoldBlock + threadIdx.x) * W; e < e1;
@@ -418,8 +417,7 @@ __global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, i
     if (e + W <= e1) {
       O y[W];
       fold<T, O, NS>(y, src, nsrc, e, scale, &sq);
-      if (stay) store<false>(out + e, y);
-      else store(out + e, y);
+      store<false>(out + e, y);
     } else {
       for (size_t i = e; i < e1; ++i) out[i] = fold_one<T, O>(src, nsrc, i, scale, &sq);
     }
@@ -429,11 +427,12 @@ __global__ __launch_bounds__(kFoldBlock) void k_grad_fold(O* out, Sources src, i
 
 // The burst form of pgk_reduce_multi (pgk_reduce.hip) for gradients: every
 // thread folds TILES vectors, reads only, and stores them at the end, so the
-// chip reads and then writes.  6.5 TB/s against 5.9 for 8 sources x 64 MiB of
-// equal types; it does not pay below 5 sources, nor where the output is wider
-// (4 sources 5.8 to 6.0 against 6.3; 8 bf16 sources to f32 5.3 against 6.4).  Its
-// stores come in one burst and cost the same with the default policy, which leaves
-// the output to what follows (with a clip 117 against 122 us for 8 x 64 MiB).
+// chip reads and then writes.  8 sources x 64 MiB of equal types, called one behind
+// the other: 95.3 us (6.3 TB/s) against 110 a vector at a time (f32 95.0, 106.6); the
+// sum is 2.2 us of it.  (rocprofv3 traces the kernel at 111 us; no timing outside it,
+// in a row or alone, shows that.)  It does not pay below 5 sources (4 of 64 MiB 58.5
+// against 57.2, 2 51 against 37.5), nor where the output is wider (8 bf16 sources to
+// f32 126 against 117, 4 f16 sources 138 against 107).
 constexpr int kBurstBlock = 256;
 template <typename T, int NS, int TILES>
 __global__ __launch_bounds__(kBurstBlock) void k_grad_fold_burst(T* out, Sources src, size_t e0, size_t e1,
@@ -737,11 +736,10 @@ int fold_t(void* out, const Sources& src, int nsrc, size_t n, double scale, doub
     constexpr size_t per = (size_t)kFoldBlock * kWidth<O>;
     const size_t tiles = (n - e0 + per - 1) / per;
     const unsigned grid = one ? 1 : tiles < (size_t)kMaxParts ? (unsigned)tiles : kMaxParts;
-    const int stay = parts && n * sizeof(O) <= kInfinityCache;
     switch (nsrc) {
 #define PGK_FOLD_CASE(NS, K) \
       K: hipLaunchKernelGGL((k_grad_fold<T, O, NS>), dim3(grid), dim3(kFoldBlock), 0, s, o, src, nsrc, e0, n, scale, \
-                            parts, held, stay); break;
+                            parts, held); break;
       PGK_FOLD_CASE(1, case 1) PGK_FOLD_CASE(2, case 2) PGK_FOLD_CASE(3, case 3) PGK_FOLD_CASE(4, case 4)
       PGK_FOLD_CASE(5, case 5) PGK_FOLD_CASE(6, case 6) PGK_FOLD_CASE(7, case 7) PGK_FOLD_CASE(kMaxUnrolled, default)
 #undef PGK_FOLD_CASE
