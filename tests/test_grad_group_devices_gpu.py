@@ -17,7 +17,7 @@ def connect(lib, rank, world, transport):
 
 def test_another_device_than_the_current_one(gpu, lib):
     """The workspace is allocated on the current device and the kernels run on the handle's: the two must be one.
-    The box has one GPU, so the handle is the one that says otherwise."""
+    With one GPU the handle is the one that says otherwise."""
     x = gpu.full((100,), 3.0, device="cuda")
     gp, ns, k = pgamd.tensor_list([x], pgamd.DT_F32)
     h = connect(lib, 0, 1, pgamd.PG_TRANSPORT_SELF)

@@ -4,8 +4,8 @@ profiles/grad_kernel_stats.csv and profiles/grad_pmc.txt.
 
   python3 tools/grad_profile.py passes N [NAME ...]   what is profiled: N passes of every case of
                                                       perf/operators.py (three sets of inputs in turn)
-  bash tools/grad_profile.sh                          the rocprofv3 runs, on a GPU -> gpurun_out/grad_prof/
-  python3 tools/grad_profile.py tables                the tables, from gpurun_out/grad_prof/
+  bash tools/grad_profile.sh DIR                      the rocprofv3 runs, on a GPU
+  python3 tools/grad_profile.py tables DIR            the tables, from what they left in DIR
 
 The first half of a case's passes warms up and is left out of the tables.  Cases
 follow each other with other kernels between them (their inputs are made), which is
@@ -19,7 +19,6 @@ import subprocess
 import sys
 
 ROOT = pathlib.Path(__file__).resolve().parents[1]
-PROF = ROOT / "gpurun_out" / "grad_prof"
 sys.path[:0] = [str(ROOT / "perf"), str(ROOT / "rdma-ring-collectives_amd")]
 
 
@@ -92,11 +91,11 @@ def algorithmic(case, kernel):
     return None
 
 
-def tables():
+def tables(found):
     import operators
     cases = operators.listed()
     commit = subprocess.run(["git", "rev-parse", "--short", "HEAD"], cwd=ROOT, capture_output=True, text=True).stdout.strip()
-    trace = segments(PROF / "kt_kernel_trace.csv", "Start_Timestamp")
+    trace = segments(found / "kt_kernel_trace.csv", "Start_Timestamp")
     assert len(trace) == len(cases), (len(trace), len(cases))
     with open(ROOT / "profiles" / "grad_kernel_stats.csv", "w") as f:
         w = csv.writer(f)
@@ -106,7 +105,7 @@ def tables():
                 w.writerow([case["name"], kernel, grid, len(us), f"{statistics.median(us):.2f}", f"{min(us):.2f}"])
     lines = [f"rocprofv3 --pmc at {commit}, FETCH_SIZE, WRITE_SIZE and the SQ counters in a run each, median per launch;"
              " FETCH_SIZE x 2 (gfx950 correction)"]
-    fetch, write, sq = (segments(PROF / f"{name}_counter_collection.csv", "Dispatch_Id") for name in ("fetch", "write", "sq"))
+    fetch, write, sq = (segments(found / f"{name}_counter_collection.csv", "Dispatch_Id") for name in ("fetch", "write", "sq"))
     for k, case in enumerate(cases):
         read = by_place(fetch[k], lambda r: float(r["Counter_Value"]) * 2048)
         wrote = by_place(write[k], lambda r: float(r["Counter_Value"]) * 1024)
@@ -130,7 +129,7 @@ def tables():
 if __name__ == "__main__":
     if sys.argv[1:2] == ["passes"]:
         passes(int(sys.argv[2]), sys.argv[3:])
-    elif sys.argv[1:] == ["tables"]:
-        tables()
+    elif sys.argv[1:2] == ["tables"] and len(sys.argv) == 3:
+        tables(pathlib.Path(sys.argv[2]))
     else:
         sys.exit(__doc__)

@@ -1,7 +1,8 @@
 #!/bin/bash
-# rocprofv3 passes over the cases of perf/operators.py (tools/grad_profile.py), on a GPU box
-# from the repo root -> gpurun_out/grad_prof/.  Each set of counters in a run of its own.
-out=$PWD/gpurun_out/grad_prof
+# rocprofv3 passes over the cases of perf/operators.py (tools/grad_profile.py), from the repo root.
+# Each set of counters in a run of its own.
+#   bash tools/grad_profile.sh DIR
+out=$(realpath -m "${1:?where the results go}")
 prog=$PWD/tools/grad_profile.py
 mkdir -p "$out"
 cd /tmp && export TMPDIR=/tmp
